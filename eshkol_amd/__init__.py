@@ -59,9 +59,22 @@ class HipOzakiInt8Stages(C.Structure):
                 ("s", i32), ("nbuf", i32), ("layout", i32), ("g_rows", u64), ("g_ld", u64)]
 
 
+class HipLayerNormArgs(C.Structure):
+    _fields_ = [("x", vp), ("gamma", vp), ("beta", vp), ("y", vp), ("mean", vp), ("rstd", vp),
+                ("rows", u64), ("cols", u64), ("ldx", u64), ("ldy", u64), ("epsilon", C.c_double),
+                ("dtype", i32), ("param_dtype", i32)]
+
+
+class HipLayerNormBackwardArgs(C.Structure):
+    _fields_ = [("grad_y", vp), ("x", vp), ("gamma", vp), ("mean", vp), ("rstd", vp), ("grad_residual", vp),
+                ("grad_x", vp), ("grad_gamma", vp), ("grad_beta", vp), ("rows", u64), ("cols", u64),
+                ("ld_grad_y", u64), ("ldx", u64), ("ld_grad_residual", u64), ("ld_grad_x", u64),
+                ("dtype", i32), ("param_dtype", i32), ("workspace", vp), ("workspace_bytes", u64)]
+
+
 BUF = C.POINTER(EshkolGPUBuffer)
 
-# name -> (restype, argtypes); every symbol the two public headers and the testing header declare
+# name -> (restype, argtypes); every symbol the public headers and the testing header declare
 SIGNATURES = {
     # gpu_memory.h
     "eshkol_gpu_init": (C.c_int, []),
@@ -170,6 +183,10 @@ SIGNATURES = {
     "hip_ozaki_crt_set_host_pass": (None, [C.c_int]),
     "hip_ozaki_crt_set_fused_scan": (None, [C.c_int]),
     "hip_igemm_set_prefetch": (None, [C.c_int]),
+    # gpu_hip_layers.h
+    "hip_layernorm": (C.c_int, [C.POINTER(HipLayerNormArgs), vp]),
+    "hip_layernorm_backward_workspace": (i64, [C.POINTER(HipLayerNormBackwardArgs)]),
+    "hip_layernorm_backward": (C.c_int, [C.POINTER(HipLayerNormBackwardArgs), vp]),
 }
 
 _lib = None

@@ -5,7 +5,7 @@
 
 Each source is compiled to an object under eshkol_amd/lib/obj/ and linked into
 one shared library whose exported symbols are the C ABI declared in
-include/eshkol/backend/gpu/gpu_memory.h and gpu_hip_tiers.h.
+include/eshkol/backend/gpu/gpu_memory.h, gpu_hip_tiers.h and gpu_hip_layers.h.
 """
 import os
 import re
@@ -35,6 +35,7 @@ SOURCES = [
     "ozaki_int8.hip",
     "elementwise.hip",
     "ozaki_fast.hip",
+    "layernorm.hip",
 ]
 # A device probe for the benchmark (register-only MFMA loops, a large copy): a
 # library of its own, so that the product library carries no measurement code.
@@ -243,7 +244,7 @@ def _compile(src, force):
     obj = os.path.join(OBJDIR, os.path.splitext(src)[0] + ".o")
     headers = [os.path.join(CSRC, h) for h in os.listdir(CSRC) if h.endswith(".h")]
     headers += [os.path.join(ROOT, "include", "eshkol", "backend", "gpu", h)
-                for h in ("gpu_memory.h", "gpu_hip_tiers.h", "gpu_hip_testing.h")]
+                for h in ("gpu_memory.h", "gpu_hip_tiers.h", "gpu_hip_layers.h", "gpu_hip_testing.h")]
     if not force and _newer(obj, [path] + headers):
         return obj
     cmd = [HIPCC] + COMMON + EXTRA.get(src, []) + ["-x", "hip", "-c", path, "-o", obj]
