@@ -22,6 +22,8 @@ MEM_HOST, MEM_HOST_PINNED, MEM_DEVICE, MEM_UNIFIED = 0, 1, 2, 3
 SYNC_NONE, SYNC_HOST_TO_DEVICE, SYNC_DEVICE_TO_HOST, SYNC_BIDIRECTIONAL = 0, 1, 2, 3
 DTYPE_F64, DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_I8 = 0, 1, 2, 3, 4
 
+ACT_NONE, ACT_TANH, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3, 4     # gpu_hip_layers.h
+
 u64, i64, i32, u32 = C.c_uint64, C.c_int64, C.c_int32, C.c_uint32
 vp, dp = C.c_void_p, C.POINTER(C.c_double)
 
@@ -70,6 +72,40 @@ class HipLayerNormBackwardArgs(C.Structure):
                 ("grad_x", vp), ("grad_gamma", vp), ("grad_beta", vp), ("rows", u64), ("cols", u64),
                 ("ld_grad_y", u64), ("ldx", u64), ("ld_grad_residual", u64), ("ld_grad_x", u64),
                 ("dtype", i32), ("param_dtype", i32), ("workspace", vp), ("workspace_bytes", u64)]
+
+
+class HipLinearArgs(C.Structure):
+    _fields_ = [("x", vp), ("w", vp), ("bias", vp), ("residual", vp), ("y", vp), ("pre", vp),
+                ("M", u64), ("K", u64), ("N", u64),
+                ("ldx", u64), ("ldw", u64), ("ld_residual", u64), ("ldy", u64), ("ld_pre", u64),
+                ("dtype", i32), ("param_dtype", i32), ("act", i32), ("trans_w", i32),
+                ("workspace", vp), ("workspace_bytes", u64)]
+
+
+class HipLinearBackwardArgs(C.Structure):
+    _fields_ = [("grad_y", vp), ("pre", vp), ("x", vp), ("w", vp), ("grad_x", vp), ("grad_w", vp), ("grad_bias", vp),
+                ("M", u64), ("K", u64), ("N", u64),
+                ("ld_grad_y", u64), ("ld_pre", u64), ("ldx", u64), ("ldw", u64), ("ld_grad_x", u64), ("ld_grad_w", u64),
+                ("dtype", i32), ("grad_w_dtype", i32), ("act", i32), ("trans_w", i32),
+                ("workspace", vp), ("workspace_bytes", u64)]
+
+
+class HipExpertsArgs(C.Structure):
+    _fields_ = [("x", vp), ("w", vp), ("bias", vp), ("offsets", vp), ("y", vp), ("pre", vp),
+                ("rows", u64), ("experts", u64), ("K", u64), ("N", u64),
+                ("ldx", u64), ("ldw", u64), ("w_stride", u64), ("ldy", u64), ("ld_pre", u64),
+                ("dtype", i32), ("param_dtype", i32), ("act", i32), ("trans_w", i32),
+                ("workspace", vp), ("workspace_bytes", u64)]
+
+
+class HipExpertsBackwardArgs(C.Structure):
+    _fields_ = [("grad_y", vp), ("pre", vp), ("x", vp), ("w", vp), ("offsets", vp),
+                ("grad_x", vp), ("grad_w", vp), ("grad_bias", vp),
+                ("rows", u64), ("experts", u64), ("K", u64), ("N", u64),
+                ("ld_grad_y", u64), ("ld_pre", u64), ("ldx", u64), ("ldw", u64), ("w_stride", u64),
+                ("ld_grad_x", u64), ("ld_grad_w", u64), ("grad_w_stride", u64),
+                ("dtype", i32), ("grad_w_dtype", i32), ("act", i32), ("trans_w", i32),
+                ("workspace", vp), ("workspace_bytes", u64)]
 
 
 BUF = C.POINTER(EshkolGPUBuffer)
@@ -187,6 +223,14 @@ SIGNATURES = {
     "hip_layernorm": (C.c_int, [C.POINTER(HipLayerNormArgs), vp]),
     "hip_layernorm_backward_workspace": (i64, [C.POINTER(HipLayerNormBackwardArgs)]),
     "hip_layernorm_backward": (C.c_int, [C.POINTER(HipLayerNormBackwardArgs), vp]),
+    "hip_linear_16_workspace": (i64, [C.POINTER(HipLinearArgs)]),
+    "hip_linear_16": (C.c_int, [C.POINTER(HipLinearArgs), vp]),
+    "hip_linear_backward_16_workspace": (i64, [C.POINTER(HipLinearBackwardArgs)]),
+    "hip_linear_backward_16": (C.c_int, [C.POINTER(HipLinearBackwardArgs), vp]),
+    "hip_experts_16_workspace": (i64, [C.POINTER(HipExpertsArgs)]),
+    "hip_experts_16": (C.c_int, [C.POINTER(HipExpertsArgs), vp]),
+    "hip_experts_backward_16_workspace": (i64, [C.POINTER(HipExpertsBackwardArgs)]),
+    "hip_experts_backward_16": (C.c_int, [C.POINTER(HipExpertsBackwardArgs), vp]),
 }
 
 _lib = None

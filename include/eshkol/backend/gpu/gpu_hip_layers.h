@@ -1,7 +1,10 @@
 /*
- * Layers of a feed-forward block as models train and serve it: layer norm with its
- * gradients. They stand beside the products and streaming kernels of
- * gpu_hip_tiers.h.
+ * Layers of a feed-forward block as models train and serve it: layer norm, the
+ * linear layer with bias, activation and residual in the product's epilogue, and
+ * the same layer held once per expert for rows that are grouped by expert; each
+ * with its gradients. They stand beside the products of gpu_hip_tiers.h
+ * (hip_hgemm_16, hip_bias_act_f64, the batched entry points) and have no
+ * counterpart in the reference, whose layers run on the host.
  *
  * Conventions: plain C, device pointers, arguments in a struct that the callee
  * only reads, `stream` is a hipStream_t passed as void* (NULL = the null stream).
@@ -38,6 +41,15 @@
 #ifdef __cplusplus
 extern "C" {
 #endif
+
+/* act: the activations of the linear layer and of the experts */
+enum {
+    HIP_ACT_NONE = 0,
+    HIP_ACT_TANH = 1,       /* the code hip_bias_act_f64 has for it */
+    HIP_ACT_RELU = 2,       /* derivative 0 at 0 */
+    HIP_ACT_GELU = 3,       /* z Phi(z), Phi the normal distribution's integral (no tanh form) */
+    HIP_ACT_SILU = 4        /* z / (1 + e^-z) */
+};
 
 /* ---- layer norm --------------------------------------------------------------
  * y = (x - mean) rstd gamma + beta for every row of `cols` elements,
@@ -85,6 +97,101 @@ typedef struct {
 } HipLayerNormBackwardArgs;
 int64_t hip_layernorm_backward_workspace(const HipLayerNormBackwardArgs* args);
 int hip_layernorm_backward(const HipLayerNormBackwardArgs* args, void* stream);
+
+/* ---- linear layer ------------------------------------------------------------
+ * z = x W + bias,  y = act(z) + residual,  pre = z
+ * on the matrix cores, dtype 2 (f16) or 3 (bf16), sums and epilogue in fp32, y and
+ * pre rounded once each (act is applied to the unrounded z). W is [K][N], or
+ * [N][K] with trans_w != 0. bias is of param_dtype (dtype or 1). pre is what the
+ * backward pass of an activation takes; NULL where nothing follows. y may be
+ * residual (with its pitch); no other output may overlap an input. M may be 0;
+ * M below 2^31, K and N at most 2^22. */
+typedef struct {
+    const void* x;          /* [M][K]                                              */
+    const void* w;          /* [K][N], trans_w: [N][K]                             */
+    const void* bias;       /* [N] or NULL                                         */
+    const void* residual;   /* [M][N] or NULL                                      */
+    void* y;                /* [M][N]                                              */
+    void* pre;              /* [M][N] or NULL                                      */
+    uint64_t M, K, N;
+    uint64_t ldx, ldw, ld_residual, ldy, ld_pre;
+    int32_t dtype, param_dtype, act, trans_w;
+    void* workspace;
+    uint64_t workspace_bytes;
+} HipLinearArgs;
+int64_t hip_linear_16_workspace(const HipLinearArgs* args);
+int hip_linear_16(const HipLinearArgs* args, void* stream);
+
+/* Its gradients, with dz = grad_y act'(pre):
+ *   grad_x = dz W^T,   grad_w = x^T dz (of W's shape),   grad_bias = sum over rows of dz
+ * pre is read only for act != 0. dz is rounded to dtype before it enters the two
+ * products (the operand type of the matrix cores); grad_bias, fp32, sums it
+ * unrounded. grad_w is of grad_w_dtype: dtype, or 1. The gradient of the residual
+ * is grad_y itself. Any output may be NULL, not all; M may be 0 (grad_w and
+ * grad_bias are then zeros). No output may overlap an input. */
+typedef struct {
+    const void* grad_y;     /* [M][N]                                              */
+    const void* pre;        /* [M][N], or NULL for act 0                           */
+    const void* x;          /* [M][K], may be NULL where grad_w is                 */
+    const void* w;          /* may be NULL where grad_x is                         */
+    void* grad_x;           /* [M][K] or NULL                                      */
+    void* grad_w;           /* [K][N] (trans_w: [N][K]) or NULL                    */
+    void* grad_bias;        /* [N] fp32 or NULL                                    */
+    uint64_t M, K, N;
+    uint64_t ld_grad_y, ld_pre, ldx, ldw, ld_grad_x, ld_grad_w;
+    int32_t dtype, grad_w_dtype, act, trans_w;
+    void* workspace;
+    uint64_t workspace_bytes;
+} HipLinearBackwardArgs;
+int64_t hip_linear_backward_16_workspace(const HipLinearBackwardArgs* args);
+int hip_linear_backward_16(const HipLinearBackwardArgs* args, void* stream);
+
+/* ---- the linear layer by expert -------------------------------------------------
+ * The rows of x are grouped by expert: those of expert e are offsets[e] ..
+ * offsets[e+1] - 1, and they are multiplied by W_e = w + e w_stride, with bias row
+ * e. offsets, experts + 1 of them in device memory, are read on the device (a
+ * router's output needs no trip to the host), ascending from at least 0 to at
+ * most rows; an expert may have no rows. Rows before offsets[0] and behind
+ * offsets[experts] belong to no expert: their outputs are left as they were.
+ * (Offsets that do not ascend, or lie outside 0 .. rows, give meaningless results, but no access
+ * outside the tensors.) experts at most 4096, rows below 2^31; otherwise as
+ * hip_linear_16, without a residual. w_stride 0: the experts' matrices back to back. */
+typedef struct {
+    const void* x;          /* [rows][K]                                           */
+    const void* w;          /* [experts][K][N], trans_w: [experts][N][K]           */
+    const void* bias;       /* [experts][N] or NULL                                */
+    const int32_t* offsets; /* [experts + 1]                                       */
+    void* y;                /* [rows][N]                                           */
+    void* pre;              /* [rows][N] or NULL                                   */
+    uint64_t rows, experts, K, N;
+    uint64_t ldx, ldw, w_stride, ldy, ld_pre;
+    int32_t dtype, param_dtype, act, trans_w;
+    void* workspace;
+    uint64_t workspace_bytes;
+} HipExpertsArgs;
+int64_t hip_experts_16_workspace(const HipExpertsArgs* args);
+int hip_experts_16(const HipExpertsArgs* args, void* stream);
+
+/* Its gradients, as hip_linear_backward_16 for every expert: grad_w and grad_bias
+ * of an expert without rows are zeros; rows of grad_x that belong to no expert are
+ * left as they were. */
+typedef struct {
+    const void* grad_y;     /* [rows][N]                                           */
+    const void* pre;        /* [rows][N], or NULL for act 0                        */
+    const void* x;          /* [rows][K], may be NULL where grad_w is              */
+    const void* w;          /* may be NULL where grad_x is                         */
+    const int32_t* offsets; /* [experts + 1]                                       */
+    void* grad_x;           /* [rows][K] or NULL                                   */
+    void* grad_w;           /* of w's shape, or NULL                               */
+    void* grad_bias;        /* [experts][N] fp32 or NULL                           */
+    uint64_t rows, experts, K, N;
+    uint64_t ld_grad_y, ld_pre, ldx, ldw, w_stride, ld_grad_x, ld_grad_w, grad_w_stride;
+    int32_t dtype, grad_w_dtype, act, trans_w;
+    void* workspace;
+    uint64_t workspace_bytes;
+} HipExpertsBackwardArgs;
+int64_t hip_experts_backward_16_workspace(const HipExpertsBackwardArgs* args);
+int hip_experts_backward_16(const HipExpertsBackwardArgs* args, void* stream);
 
 #ifdef __cplusplus
 }

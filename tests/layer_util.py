@@ -1,7 +1,7 @@
 """Helpers for the tests of the layer operators (gpu_hip_layers.h): element types in numpy, matrices in
 device memory with a pitch and an odd start, HIP graphs, and the plain forms in 64 bits."""
 import ctypes as C
-from math import erf
+from math import erfc
 
 import numpy as np
 
@@ -155,7 +155,7 @@ class Graph:
 
 # ---- activations in 64 bits ---------------------------------------------------------------------------
 
-_erf = np.vectorize(erf, otypes=[np.float64])
+_erfc = np.vectorize(erfc, otypes=[np.float64])         # 1 + erf would lose every digit of the lower tail
 
 
 def act(z, code):
@@ -164,7 +164,7 @@ def act(z, code):
     if code == 2:
         return np.maximum(z, 0.0)
     if code == 3:
-        return 0.5 * z * (1.0 + _erf(z / np.sqrt(2.0)))
+        return 0.5 * z * _erfc(-z / np.sqrt(2.0))
     if code == 4:
         return z / (1.0 + np.exp(-z))
     return z
@@ -176,7 +176,7 @@ def slope(z, code):
     if code == 2:
         return (z > 0).astype(np.float64)
     if code == 3:
-        return 0.5 * (1.0 + _erf(z / np.sqrt(2.0))) + z * np.exp(-0.5 * z * z) / np.sqrt(2.0 * np.pi)
+        return 0.5 * _erfc(-z / np.sqrt(2.0)) + z * np.exp(-0.5 * z * z) / np.sqrt(2.0 * np.pi)
     if code == 4:
         s = 1.0 / (1.0 + np.exp(-z))
         return s * (1.0 + z * (1.0 - s))

@@ -110,3 +110,98 @@ assert lib.hip_layernorm(C.byref(a), None) == -1
     r = run_child(body, {"ESHKOL_GPU_VERBOSE": "1"})
     assert r.returncode == 0 and "[GPU] hip_layernorm: param_dtype 2 beside dtype 3" in r.stderr, r.stderr
     assert run_child(body).stderr.count("hip_layernorm") == 0
+
+
+# ---- linear layer and experts -------------------------------------------------------------------------------
+
+def linear(**changes):
+    a = dict(x=1 << 20, w=1 << 21, bias=1 << 12, residual=1 << 22, y=1 << 23, pre=1 << 24, M=100, K=64, N=96, dtype=3, param_dtype=3, act=3)
+    a.update(changes)
+    return ea.HipLinearArgs(**a)
+
+
+def linear_back(**changes):
+    a = dict(grad_y=1 << 20, pre=1 << 21, x=1 << 22, w=1 << 23, grad_x=1 << 24, grad_w=1 << 25, grad_bias=1 << 26, M=100, K=64, N=96, dtype=3, grad_w_dtype=3, act=3)
+    a.update(changes)
+    return ea.HipLinearBackwardArgs(**a)
+
+
+def experts(**changes):
+    a = dict(x=1 << 20, w=1 << 21, bias=1 << 12, offsets=1 << 10, y=1 << 23, pre=1 << 24, rows=100, experts=4, K=64, N=96, dtype=2, param_dtype=1, act=4)
+    a.update(changes)
+    return ea.HipExpertsArgs(**a)
+
+
+def experts_back(**changes):
+    a = dict(grad_y=1 << 20, pre=1 << 21, x=1 << 22, w=1 << 23, offsets=1 << 10, grad_x=1 << 24, grad_w=1 << 25, grad_bias=1 << 26, rows=100, experts=4, K=64, N=96,
+             dtype=2, grad_w_dtype=1, act=4)
+    a.update(changes)
+    return ea.HipExpertsBackwardArgs(**a)
+
+
+SIZES_REFUSED = [dict(K=0), dict(N=0), dict(K=(1 << 22) + 1), dict(N=(1 << 22) + 1), dict(dtype=0), dict(dtype=1), dict(dtype=4), dict(act=5), dict(act=-1)]
+FORWARD_REFUSED = SIZES_REFUSED + [dict(x=None), dict(w=None), dict(y=None), dict(x=ODD), dict(w=ODD), dict(y=ODD), dict(pre=ODD), dict(ldx=63), dict(ldw=95),
+                                   dict(ldw=63, trans_w=1), dict(ldy=95), dict(ld_pre=95), dict(param_dtype=0), dict(y=1 << 20), dict(y=1 << 21), dict(pre=1 << 23),
+                                   dict(pre=1 << 20), dict(pre=1 << 21)]
+BACKWARD_REFUSED = SIZES_REFUSED + [dict(grad_y=None), dict(pre=None), dict(x=None), dict(w=None), dict(grad_x=None, grad_w=None, grad_bias=None), dict(grad_y=ODD), dict(pre=ODD),
+                                    dict(x=ODD), dict(w=ODD), dict(grad_x=ODD), dict(grad_w=ODD), dict(grad_bias=0x10002), dict(ld_grad_y=95), dict(ld_pre=95), dict(ldx=63),
+                                    dict(ldw=95), dict(ld_grad_x=63), dict(ld_grad_w=95), dict(grad_w_dtype=0), dict(grad_x=1 << 20), dict(grad_w=1 << 23), dict(grad_bias=1 << 25)]
+EXPERTS_REFUSED = [dict(experts=0), dict(experts=4097), dict(offsets=None), dict(offsets=ODD), dict(rows=1 << 31), dict(w_stride=64 * 96 - 1)]
+KINDS = {"hip_linear_16": (linear, FORWARD_REFUSED + [dict(M=1 << 31), dict(bias=ODD), dict(param_dtype=2), dict(residual=ODD), dict(ld_residual=95), dict(pre=1 << 22), dict(y=1 << 22, ldy=104)]),
+         "hip_linear_backward_16": (linear_back, BACKWARD_REFUSED + [dict(M=1 << 31), dict(grad_w_dtype=2)]),
+         "hip_experts_16": (experts, FORWARD_REFUSED + EXPERTS_REFUSED + [dict(bias=0x10002), dict(param_dtype=3)]),
+         "hip_experts_backward_16": (experts_back, BACKWARD_REFUSED + EXPERTS_REFUSED + [dict(grad_w_stride=100), dict(grad_w_dtype=3)])}
+
+
+@pytest.mark.parametrize("name,change", [(n, c) for n, (_, cs) in KINDS.items() for c in cs], ids=str)
+def test_refuses(name, change):
+    lib = ea.load()
+    a = KINDS[name][0](**change)
+    assert getattr(lib, name + "_workspace")(C.byref(a)) == -1
+    assert getattr(lib, name)(C.byref(a), None) == -1
+
+
+@pytest.mark.parametrize("name", list(KINDS))
+def test_accepts_and_says_what_it_needs(name):
+    lib = ea.load()
+    make, size, entry = KINDS[name][0], getattr(lib, name + "_workspace"), getattr(lib, name)
+    assert size(None) == -1 and entry(None, None) == -1
+    need = size(C.byref(make()))
+    assert need >= 0
+    rows = "M" if "linear" in name else "rows"
+    assert size(C.byref(make(**{rows: 0}))) == 0                 # no rows: nothing to hold
+    # operands off 16-byte boundaries are copied for the tiled kernel (a few rows are read as they are)
+    assert size(C.byref(make(ldx=67, **{rows: 1000}))) > size(C.byref(make(**{rows: 1000})))
+    if "backward" in name:
+        assert need > 0
+    if need:
+        for given in (dict(), dict(workspace=1 << 27, workspace_bytes=need - 1), dict(workspace=(1 << 27) + 8, workspace_bytes=need)):
+            assert entry(C.byref(make(**given)), None) == -2
+
+
+def test_forward_without_rows_needs_nothing():
+    lib = ea.load()
+    assert lib.hip_linear_16(C.byref(linear(M=0, x=None, w=None, y=None)), None) == 0
+    assert lib.hip_experts_16(C.byref(experts(rows=0, x=None, w=None, y=None, offsets=None)), None) == 0
+    assert lib.hip_linear_16(C.byref(linear(M=0, N=0)), None) == -1
+
+
+def test_optional_arguments():
+    lib = ea.load()
+    assert lib.hip_linear_16_workspace(C.byref(linear(bias=None, residual=None, pre=None))) >= 0
+    assert lib.hip_linear_backward_16_workspace(C.byref(linear_back(act=0, pre=None))) >= 0
+    assert lib.hip_linear_backward_16_workspace(C.byref(linear_back(grad_w=None, x=None))) >= 0
+    assert lib.hip_linear_backward_16_workspace(C.byref(linear_back(grad_x=None, w=None))) >= 0
+    assert lib.hip_experts_backward_16_workspace(C.byref(experts_back(grad_x=None, w=None))) >= 0
+
+
+def test_the_derivatives_the_gpu_tests_use_are_the_activations_own():
+    """Central differences of a step of 1e-5: off by the third derivative (at most 2) times 1e-10 / 6 and by the
+    rounding of two values up to 6 over 2e-5."""
+    import numpy as np
+    from layer_util import act, slope
+    z = np.concatenate([np.linspace(-6, 6, 997), [1e-3, -1e-3]])
+    for code in (1, 2, 3, 4):
+        d = (act(z + 1e-5, code) - act(z - 1e-5, code)) / 2e-5
+        far = np.abs(z) > 1e-4 if code == 2 else np.ones_like(z, bool)
+        assert np.abs(d - slope(z, code))[far].max() < 1e-10 + 8 * 6 * 2.0 ** -53 / 1e-5, code
