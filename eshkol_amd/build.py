@@ -37,6 +37,8 @@ SOURCES = [
     "ozaki_fast.hip",
     "layernorm.hip",
     "linear_16.hip",
+    "linear_16_bf16.hip",
+    "linear_16_f16.hip",
 ]
 # A device probe for the benchmark (register-only MFMA loops, a large copy): a
 # library of its own, so that the product library carries no measurement code.
@@ -70,7 +72,7 @@ COMMON = [
 NO_SPILL = {"igemm_i8.hip": ["igemm_i8_direct_kernel", "igemm_i8_direct_half_kernel"], "hgemm_16.hip": ["hgemm_direct_kernel"]}
 # Sources whose asm statements load into LDS only: no register arrives late, so spills do
 # no harm, but the scalar operands of those loads are scanned as well.
-ASM_TO_LDS = ["linear_16.hip"]
+ASM_TO_LDS = ["linear_16_bf16.hip", "linear_16_f16.hip"]
 
 
 def _check_no_spill(src, remarks):

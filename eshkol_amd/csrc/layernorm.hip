@@ -339,6 +339,7 @@ void norm_join_kernel(const Acc* __restrict__ part, uint32_t n, uint32_t cols, A
     const uint32_t s = threadIdx.x >> 5;
     Acc sum = 0;
     if (c < cols)
+#pragma unroll 8
         for (uint32_t p = s; p < n; p += 8) sum += part[((uint64_t)p * 2 + blockIdx.y) * cols + c];
     tile[s][threadIdx.x & 31] = sum;
     __syncthreads();

@@ -8,6 +8,8 @@
 
 #include "layer_common.h"
 
+#include <algorithm>
+
 /* How an operand lies in memory: its rows (m or n) apart and k contiguous, or k
  * apart and the rows contiguous. */
 enum { ROWS_K = 0, K_ROWS = 1 };
@@ -38,7 +40,77 @@ struct LinearArgs {
     uint32_t experts;
     uint64_t b_stride, y_stride;   /* elements per expert: B (GROUP_ROWS), C (GROUP_K) */
     uint32_t tiles_m, tiles_n;
+    uint32_t wg_tiles;          /* workgroups of one part: the tiles, rounded up to a multiple of 8 */
 };
+
+namespace linear {
+
+/* dz = grad_y act'(pre), and the sums of dz's columns before it is rounded. A workgroup takes 256 columns (32 threads, eight
+ * each) of every parts-th eight rows of its expert; its eight rows of threads are joined in LDS. */
+struct SlopeArgs {
+    const uint16_t *dy, *pre;
+    uint16_t* dz;               /* NULL: the sums alone                            */
+    float* part;                /* [experts][parts][N], or NULL                    */
+    uint64_t ld_dy, ld_pre, ld_dz;
+    uint32_t rows, N, parts, experts, across, blocks;      /* across: workgroups per row of parts */
+    const int32_t* offsets;
+    int act;
+};
+
+/* The sums of a bias gradient's parts, in ascending order: a thread takes a column of an expert. */
+struct BiasJoin {
+    const float* part;          /* [experts][parts][N]                             */
+    float* out;                 /* [experts][N]                                    */
+    uint32_t N, parts, experts;
+};
+
+/* Rows that do not start on 16-byte boundaries, or are no multiple of 16 bytes, copied to ones that do and are (zeros
+ * behind their end): `chunks` pieces of 16 bytes of matrices of rows x cols. */
+struct AlignArgs {
+    const uint16_t* in;
+    uint16_t* out;
+    uint64_t ld, stride, rows, chunks;
+    uint32_t cols, out_ld, blocks;
+};
+
+/* A matrix operand as the caller gave it, and whether it has to be copied before the tiled kernel may read it. */
+struct Matrix {
+    const uint16_t* p;
+    uint64_t ld, stride, rows, cols, count;
+    bool copy;
+    uint64_t copy_bytes;
+};
+
+/* What a product is: C[M][N] over K; per expert where group says so. */
+struct Shape {
+    int fa, fb, group;
+    uint64_t M, N, K, experts;
+};
+enum { TILE_LARGE, TILE_WIDE, TILE_SQUARE };
+
+struct Product {
+    Shape s;
+    Matrix a, b;
+    LinearArgs g;
+    bool thin;
+    int rt;
+    uint32_t splits, part_k, part_ld;
+    uint64_t part_bytes;
+    uint64_t copy_bytes() const { return thin ? 0 : a.copy_bytes + b.copy_bytes; }
+};
+
+inline uint32_t tiles_of(uint64_t n, uint32_t t) { return (uint32_t)((n + t - 1) / t); }
+inline uint64_t tile_count(const Shape& s, uint32_t bm, uint32_t bn) {
+    uint64_t m = tiles_of(s.M, bm);
+    if (s.group == GROUP_ROWS) m += std::min(s.experts, s.M);               /* each group may end inside a tile */
+    return m * tiles_of(s.N, bn) * (s.group == GROUP_K ? s.experts : 1);
+}
+
+/* Queues one or two products with what goes before and behind them (linear_16.h), for one element type each. */
+int run_bf16(Product* q, int n, int tile, const SlopeArgs* slope, const BiasJoin* bias, char* ws, hipStream_t st);
+int run_f16(Product* q, int n, int tile, const SlopeArgs* slope, const BiasJoin* bias, char* ws, hipStream_t st);
+
+}  // namespace linear
 
 #ifdef __HIPCC__
 namespace linear {
@@ -92,24 +164,49 @@ __device__ __forceinline__ float tanh_of(float z) {
 }
 __device__ __forceinline__ float sigmoid_of(float z) { return __builtin_amdgcn_rcpf(1.0f + exp_of(-z)); }
 
-__device__ __forceinline__ float act_of(float z, int act) {
+/* z no further out than +-most, where the functions below have long reached their limits, so that an infinity gives
+ * the limit and not infinity times 0; NaN stays NaN */
+__device__ __forceinline__ float within(float z, float most) { return fabsf(z) > most ? __builtin_copysignf(most, z) : z; }
+
+/* z Phi(z) = max(z, 0) - |z| Phi(-|z|), Phi(-a) = exp(-a^2 / 2) (c1 t + ... + c6 t^6), t = 1 / (1 + p a): p and the
+ * coefficients were fitted for the least relative error, 3.7e-6 over 0 <= a <= 13.5 (where Phi leaves the range of
+ * fp32). That is 1/130 of half a step of f16, and half the instructions of the complement above: an epilogue's
+ * vector work is not hidden behind the matrix cores of the same wave. */
+__device__ __forceinline__ float gelu_of(float z) {
+    const float a = fabsf(z) > 14.0f ? 14.0f : fabsf(z);
+    const float t = __builtin_amdgcn_rcpf(fmaf(a, 0.3076693545535144f, 1.0f));
+    float p = -0.0758072764114048f;
+    p = fmaf(p, t, 0.19153177722556594f);
+    p = fmaf(p, t, 0.0054149948373767845f);
+    p = fmaf(p, t, 0.1372896528609662f);
+    p = fmaf(p, t, 0.11856265887668457f);
+    p = fmaf(p, t, 0.1230063487838367f);
+    return fmaf(-a, p * t * __builtin_amdgcn_exp2f(a * a * -0.72134752044448170f), fmaxf(z, 0.0f));
+}
+
+/* eight activations: the choice is made once for all of them */
+__device__ __forceinline__ void act8(float (&v)[8], int act) {
+#define EACH(expr) do { _Pragma("unroll") for (int i = 0; i < 8; i++) { const float z = v[i]; v[i] = (expr); } } while (0)
     switch (act) {
-    case HIP_ACT_TANH: return tanh_of(z);
-    case HIP_ACT_RELU: return z < 0.0f ? 0.0f : z;              /* NaN stays NaN */
-    case HIP_ACT_GELU: return z * normal_integral(z);
-    case HIP_ACT_SILU: return z * sigmoid_of(z);
-    default: return z;
+    case HIP_ACT_TANH: EACH(tanh_of(z)); break;
+    case HIP_ACT_RELU: EACH(z < 0.0f ? 0.0f : z); break;        /* NaN stays NaN */
+    case HIP_ACT_GELU: EACH(gelu_of(z)); break;
+    case HIP_ACT_SILU: EACH((z < -100.0f ? -100.0f : z) * sigmoid_of(z)); break;
+    default: break;
     }
 }
-/* its derivative */
-__device__ __forceinline__ float slope_of(float z, int act) {
+/* d times the derivatives at z */
+__device__ __forceinline__ void slope8(float (&d)[8], const float (&v)[8], int act) {
+#define SLOPE(expr) do { _Pragma("unroll") for (int i = 0; i < 8; i++) { const float z = v[i]; d[i] *= (expr); } } while (0)
     switch (act) {
-    case HIP_ACT_TANH: { const float t = tanh_of(z); return fmaf(-t, t, 1.0f); }
-    case HIP_ACT_RELU: return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
-    case HIP_ACT_GELU: return fmaf(z * 0.39894228040143268f, exp_of(-0.5f * z * z), normal_integral(z));
-    case HIP_ACT_SILU: { const float s = sigmoid_of(z); return s * fmaf(z, 1.0f - s, 1.0f); }
-    default: return 1.0f;
+    case HIP_ACT_TANH: SLOPE(({ const float t = tanh_of(z); fmaf(-t, t, 1.0f); })); break;
+    case HIP_ACT_RELU: SLOPE(z > 0.0f ? 1.0f : (z != z ? z : 0.0f)); break;
+    case HIP_ACT_GELU: SLOPE(({ const float c = within(z, 14.0f); fmaf(c * 0.39894228040143268f, exp_of(-0.5f * c * c), normal_integral(c)); })); break;
+    case HIP_ACT_SILU: SLOPE(({ const float c = within(z, 100.0f), s = sigmoid_of(c); s * fmaf(c, 1.0f - s, 1.0f); })); break;
+    default: break;
     }
+#undef SLOPE
+#undef EACH
 }
 
 /* the group of an expert, inside 0 .. rows whatever the offsets hold */
@@ -142,10 +239,7 @@ __device__ __forceinline__ void finish_row8(const LinearEpilogue& e, void* y_at,
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] += bias[i];
     if (e.pre) store_row<E, float, 8>((E*)e.pre + row * e.ld_pre, c, N, v);
-    if (e.act) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = act_of(v[i], e.act);
-    }
+    act8(v, e.act);
     if (e.residual) {
         float r[8];
         load_row<E, float, 8>((const E*)e.residual + row * e.ld_res, c, N, r);

@@ -4,7 +4,8 @@ both (gpu_hip_layers.h), against the formulas in 64 bits on the same inputs.
 Tolerances, u = 2^-24. Products of two 16-bit values are exact in fp32; n of them are added in some order, each addition
 off by at most 2 u of the running sum (whether the matrix cores round or cut): 2 (n + 8) u times the sum of magnitudes.
 The activations are off by u (24 + 2 |z| + 2 z^2) relative (an exponential's argument is off by u of itself; the
-argument is z or z^2 / 2) and pass an error of z on by at most 1.13. A rounding to the output's type is off by half a
+argument is z or z^2 / 2), gelu by 3.7e-6 = 62 u more (the fit of the normal integral that its kernel states), and pass
+an error of z on by at most 1.13. A rounding to the output's type is off by half a
 step. dz enters the products rounded to the 16-bit type (half a step of each value) unless there is no activation."""
 import ctypes as C
 import os
@@ -25,7 +26,7 @@ ACTS = [0, 1, 2, 3, 4]
 
 
 def act_error(z, code):
-    return 0.0 if code in (0, 2) else U * (24 + 2 * np.abs(z) + 2 * z * z)
+    return 0.0 if code in (0, 2) else U * (24 + (62 if code == 3 else 0) + 2 * np.abs(z) + 2 * z * z)
 
 
 class Layer:
@@ -209,6 +210,30 @@ def test_activations_far_out(gpu, code):
         t.pre = Mat((3, N), BF16, values=np.broadcast_to(z, (3, N)))
     _, _, gb = t.backward(want="b")
     t.check_backward(None, None, gb)
+
+
+def test_activations_at_the_ends_of_the_range(gpu):
+    """Sums of +-infinity, of the type's largest value and NaN: the limits, and NaN."""
+    big = 3.3895313892515355e38
+    z = np.array([np.inf, -np.inf, big, -big, np.nan, 200.0, -200.0, 14.0, -14.0])
+    limits = {0: z, 1: np.array([1, -1, 1, -1, np.nan, 1, -1, 1, -1]), 2: np.array([np.inf, 0, big, 0, np.nan, 200, 0, 14, 0])}
+    limits[3] = limits[4] = limits[2]
+    flat = {0: z * 0 + 1, 1: z * 0, 2: np.array([1, 0, 1, 0, np.nan, 1, 0, 1, 0])}
+    flat[0][:], flat[1][[0, 1, 2, 3]] = 1, 0
+    flat[3] = flat[4] = flat[2]
+    for code in ACTS:
+        for M in (4, 70):
+            t = Layer(M, 8, len(z), BF16, 0, code, F32)
+            t.x = Mat((M, 8), BF16, values=np.zeros((M, 8)))
+            t.bias = vec(z[None], F32)
+            y = t.forward()[0].get()
+            close(y, np.broadcast_to(limits[code], y.shape), 1.2e-5 + HALF[BF16] * np.abs(limits[code][np.isfinite(limits[code])]).max() * (np.abs(y) > 1e30), "act %d" % code)
+        if code:
+            t = Layer(1, 8, len(z), BF16, 0, code, F32)
+            t.dy = Mat((1, len(z)), BF16, values=np.ones((1, len(z))))
+            t.pre = Mat((1, len(z)), BF16, values=z[None])
+            got = t.backward(want="b")[2].get()
+            close(got, flat[code][None], 1.2e-5, "slope %d" % code)
 
 
 def test_infinities_and_nan_reach_their_rows_and_columns_alone(gpu):
