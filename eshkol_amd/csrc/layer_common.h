@@ -51,10 +51,10 @@ template <class T> struct Vec16 {
     typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
 };
 
-/* elements c .. c + N - 1 of a row of n, zeros beyond its end */
-template <class T, class Acc, int N>
+/* elements c .. c + N - 1 of a row of n, zeros beyond its end; EVEN: the caller knows that they are all there */
+template <class T, class Acc, int N, bool EVEN = false>
 __device__ __forceinline__ void load_row(const T* row, uint32_t c, uint32_t n, Acc (&out)[N]) {
-    if (c + N <= n) {
+    if (EVEN || c + N <= n) {
         typedef T vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
         const vec v = *(const vec*)(row + c);
 #pragma unroll
@@ -65,14 +65,15 @@ __device__ __forceinline__ void load_row(const T* row, uint32_t c, uint32_t n, A
     }
 }
 
-template <class T, class Acc, int N>
+template <class T, class Acc, int N, bool STREAM = false>
 __device__ __forceinline__ void store_row(T* row, uint32_t c, uint32_t n, const Acc (&in)[N]) {
     if (c + N <= n) {
         typedef T vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
         vec v;
 #pragma unroll
         for (int e = 0; e < N; e++) v[e] = (T)in[e];
-        *(vec*)(row + c) = v;
+        if constexpr (STREAM) __builtin_nontemporal_store(v, (vec*)(row + c));
+        else *(vec*)(row + c) = v;
     } else {
 #pragma unroll
         for (int e = 0; e < N; e++) if (c + e < n) row[c + e] = (T)in[e];
@@ -80,13 +81,13 @@ __device__ __forceinline__ void store_row(T* row, uint32_t c, uint32_t n, const 
 }
 
 /* a parameter vector of type T, or of fp32 where wide != 0; `none` for a NULL one */
-template <class T, class Acc, int N>
+template <class T, class Acc, int N, bool EVEN = false>
 __device__ __forceinline__ void load_param(const void* p, int wide, Acc none, uint32_t c, uint32_t n, Acc (&out)[N]) {
     if (!p) {
 #pragma unroll
         for (int e = 0; e < N; e++) out[e] = none;
-    } else if (wide) load_row<float, Acc, N>((const float*)p, c, n, out);
-    else load_row<T, Acc, N>((const T*)p, c, n, out);
+    } else if (wide) load_row<float, Acc, N, EVEN>((const float*)p, c, n, out);
+    else load_row<T, Acc, N, EVEN>((const T*)p, c, n, out);
 }
 
 template <class Acc> __device__ __forceinline__ Acc fma_of(Acc a, Acc b, Acc c);

@@ -44,9 +44,55 @@ __device__ __forceinline__ Acc team_sum(Acc v, Acc (*scratch)[T / 64 > 0 ? T / 6
     return v;
 }
 
-/* A row is held by T threads, V vectors of 16 bytes each (T = 64: four rows per
- * workgroup, one per wave). */
-template <int DT, int T, int V>
+/* Sixteen bytes of a row, kept as four words: a vector of 16-bit elements that lives across a branch is taken apart into a
+ * register for each element. */
+typedef int words_t __attribute__((ext_vector_type(4)));
+template <class E> __device__ __forceinline__ typename Vec16<E>::type elements(words_t w) { return __builtin_bit_cast(typename Vec16<E>::type, w); }
+/* element e, widened */
+template <class E> __device__ __forceinline__ auto wide_of(words_t w, int e) {
+    if constexpr (sizeof(E) == 8) return (double)elements<E>(w)[e];
+    else if constexpr (__is_same(E, __bf16)) return __int_as_float((e & 1) ? (w[e >> 1] & (int)0xffff0000) : (w[e >> 1] << 16));
+    else return (float)elements<E>(w)[e];
+}
+
+/* One 16-byte vector of a row from element c on, zeros behind the row's end. EVEN: rows are whole vectors. */
+template <class E, bool EVEN>
+__device__ __forceinline__ words_t load_vec(const E* row, uint32_t c, uint32_t n) {
+    typedef int unaligned __attribute__((ext_vector_type(4), aligned(2)));     /* global memory takes it at any address */
+    constexpr int N = Vec16<E>::N;
+    words_t v = {0, 0, 0, 0};
+    if (EVEN ? c < n : c + N <= n) v = *(const unaligned*)(row + c);
+    else if (!EVEN && c < n) {
+        typename Vec16<E>::type part = {};
+#pragma unroll
+        for (int e = 0; e < N; e++) if (c + e < n) part[e] = row[c + e];
+        v = __builtin_bit_cast(words_t, part);
+    }
+    return v;
+}
+/* Makes the compiler take a vector's values as new ones: it would otherwise keep the widened copies of one sweep for the
+ * next, in twice the registers. It also keeps the loads behind it (the parameters of this vector) from being moved up in
+ * front of the sweep, all of a row's at once. */
+/* A thread's place in its row, as a value of this turn of the loop: the addresses of every vector and parameter would
+ * otherwise be computed once and kept, in more registers than the row itself. */
+__device__ __forceinline__ int position(int t) { asm volatile("" : "+v"(t)); return t; }
+__device__ __forceinline__ void renew(words_t& w) { asm volatile("" : "+v"(w) :: "memory"); }
+
+template <class E, class Acc, bool EVEN>
+__device__ __forceinline__ void store_vec(E* row, uint32_t c, uint32_t n, const Acc (&in)[Vec16<E>::N]) {
+    if constexpr (EVEN) {
+        typedef typename Vec16<E>::type vec;
+        vec v;
+#pragma unroll
+        for (int e = 0; e < Vec16<E>::N; e++) v[e] = (E)in[e];
+        if (c < n) *(vec*)(row + c) = v;
+    } else store_row<E, Acc, Vec16<E>::N>(row, c, n, in);
+}
+
+/* A row is held by T threads, V vectors of 16 bytes each, as it lies in memory: it is widened again for each of the three
+ * sweeps, which costs less than the registers of a wide copy (32768 x 4096 bf16: 117 registers and 166 us with one). T = 64: a row
+ * per wave, no barrier. The next row is requested before the current one is worked on. */
+template <int DT, int T, int V, bool EVEN>
 __global__ __launch_bounds__(T < 256 ? 256 : T)
 void norm_kernel(NormArgs a) {
     typedef typename Elem<DT>::T E;
@@ -54,28 +100,37 @@ void norm_kernel(NormArgs a) {
     constexpr int N = Vec16<E>::N;
     constexpr int PER = T < 256 ? 256 / T : 1;              /* rows per workgroup */
     __shared__ Acc scratch[2][T / 64 > 0 ? T / 64 : 1];
-    const int t = threadIdx.x % T;
+    const int t0 = threadIdx.x % T;
     const Acc inv_n = (Acc)1 / (Acc)a.cols;
-    for (uint64_t row = (uint64_t)blockIdx.x * PER + threadIdx.x / T; row < a.rows; row += (uint64_t)gridDim.x * PER) {
-        const E* xr = (const E*)a.x + row * a.ldx;
-        Acc v[V][N];
+    const uint64_t step = (uint64_t)gridDim.x * PER;
+    uint64_t row = (uint64_t)blockIdx.x * PER + threadIdx.x / T;
+    if (row >= a.rows) return;                              /* whole waves; whole workgroups where they share a row */
+    words_t x[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) x[i] = load_vec<E, EVEN>((const E*)a.x + row * a.ldx, (uint32_t)(t0 + i * T) * N, a.cols);
+    for (; row < a.rows; row += step) {
+        const int t = position(t0);
+        words_t next[V];
+        const uint64_t ahead = row + step < a.rows ? row + step : row;
+#pragma unroll
+        for (int i = 0; i < V; i++) next[i] = load_vec<E, EVEN>((const E*)a.x + ahead * a.ldx, (uint32_t)(t + i * T) * N, a.cols);
         Acc s = 0;
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-            load_row<E, Acc, N>(xr, (uint32_t)(t + i * T) * N, a.cols, v[i]);
-#pragma unroll
-            for (int e = 0; e < N; e++) s += v[i][e];
-        }
-        const Acc mean = team_sum<T, Acc>(s, scratch, 0) * inv_n;
-        Acc q = 0;
 #pragma unroll
         for (int i = 0; i < V; i++)
 #pragma unroll
+            for (int e = 0; e < N; e++) s += wide_of<E>(x[i], e);
+        const Acc mean = team_sum<T, Acc>(s, scratch, 0) * inv_n;
+        Acc q = 0;
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            renew(x[i]);
+#pragma unroll
             for (int e = 0; e < N; e++) {
-                const Acc d = (uint32_t)(t + i * T) * N + e < a.cols ? v[i][e] - mean : (Acc)0;
-                v[i][e] = d;
+                const uint32_t c = (uint32_t)(t + i * T) * N + (EVEN ? 0 : e);
+                const Acc d = c < a.cols ? wide_of<E>(x[i], e) - mean : (Acc)0;
                 q = fma_of(d, d, q);
             }
+        }
         const Acc rstd = (Acc)1 / (Acc)sqrt(fma_of(team_sum<T, Acc>(q, scratch, 1), inv_n, (Acc)a.epsilon));
         if (t == 0) {
             if (a.mean) ((Acc*)a.mean)[row] = mean;
@@ -85,13 +140,16 @@ void norm_kernel(NormArgs a) {
 #pragma unroll
         for (int i = 0; i < V; i++) {
             const uint32_t c = (uint32_t)(t + i * T) * N;
-            if (c >= a.cols) continue;
-            Acc g[N], b[N];
-            load_param<E, Acc, N>(a.gamma, a.wide, (Acc)1, c, a.cols, g);
-            load_param<E, Acc, N>(a.beta, a.wide, (Acc)0, c, a.cols, b);
+            renew(x[i]);
+            if (c < a.cols) {
+                Acc g[N], b[N], o[N];
+                load_param<E, Acc, N, EVEN>(a.gamma, a.wide, (Acc)1, c, a.cols, g);
+                load_param<E, Acc, N, EVEN>(a.beta, a.wide, (Acc)0, c, a.cols, b);
 #pragma unroll
-            for (int e = 0; e < N; e++) v[i][e] = fma_of(v[i][e] * rstd, g[e], b[e]);
-            store_row<E, Acc, N>(yr, c, a.cols, v[i]);
+                for (int e = 0; e < N; e++) o[e] = fma_of((wide_of<E>(x[i], e) - mean) * rstd, g[e], b[e]);
+                store_vec<E, Acc, EVEN>(yr, c, a.cols, o);
+            }
+            x[i] = next[i];
         }
     }
 }
@@ -150,9 +208,10 @@ struct NormBackArgs {
     int wide;
 };
 
-/* T threads per row as above. Each thread adds grad_y h and grad_y of its columns
- * over the rows it sees; with T = 64 the four waves' sums are joined in LDS at the end. */
-template <int DT, int T, int V>
+/* T threads per row and V vectors per thread as above, the next row's values requested before the current row is
+ * worked on. Each thread adds grad_y h and grad_y of its columns over the rows it sees; with T = 64 the four waves'
+ * sums are joined in LDS at the end. */
+template <int DT, int T, int V, bool EVEN>
 __global__ __launch_bounds__(T < 256 ? 256 : T)
 void norm_back_kernel(NormBackArgs a) {
     typedef typename Elem<DT>::T E;
@@ -162,77 +221,95 @@ void norm_back_kernel(NormBackArgs a) {
     constexpr int W = T / 64 > 0 ? T / 64 : 1;
     __shared__ Acc scratch[2][2][W];
     __shared__ Acc join[PER > 1 ? PER : 1][PER > 1 ? T * V * N : 1];
-    const int t = threadIdx.x % T;
+    const int t0 = threadIdx.x % T;
     const Acc inv_n = (Acc)1 / (Acc)a.cols;
+    const uint64_t step = (uint64_t)gridDim.x * PER;
+    uint64_t row = (uint64_t)blockIdx.x * PER + threadIdx.x / T;
     Acc sg[V][N], sb[V][N];
 #pragma unroll
     for (int i = 0; i < V; i++)
 #pragma unroll
         for (int e = 0; e < N; e++) sg[i][e] = sb[i][e] = 0;
+    words_t x[V], d[V], r[V];
+    Acc mean = 0, rstd = 0;
+    auto load = [&](int t, uint64_t at, words_t (&xv)[V], words_t (&dv)[V], words_t (&rv)[V], Acc& m, Acc& s) {
+        m = ((const Acc*)a.mean)[at];
+        s = ((const Acc*)a.rstd)[at];
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const uint32_t c = (uint32_t)(t + i * T) * N;
+            xv[i] = load_vec<E, EVEN>((const E*)a.x + at * a.ldx, c, a.cols);
+            dv[i] = load_vec<E, EVEN>((const E*)a.dy + at * a.ld_dy, c, a.cols);
+            if (a.res) rv[i] = load_vec<E, EVEN>((const E*)a.res + at * a.ld_res, c, a.cols);
+        }
+    };
+    if (row < a.rows) load(t0, row, x, d, r, mean, rstd);
     int turn = 0;
-    for (uint64_t row = (uint64_t)blockIdx.x * PER + threadIdx.x / T; row < a.rows; row += (uint64_t)gridDim.x * PER, turn ^= 1) {
-        const E* xr = (const E*)a.x + row * a.ldx;
-        const E* dr = (const E*)a.dy + row * a.ld_dy;
-        const Acc mean = ((const Acc*)a.mean)[row], rstd = ((const Acc*)a.rstd)[row];
-        Acc h[V][N], d[V][N];
+    for (; row < a.rows; row += step, turn ^= 1) {
+        const int t = position(t0);
+        words_t nx[V], nd[V], nr[V];
+        Acc nmean, nrstd;
+        load(t, row + step < a.rows ? row + step : row, nx, nd, nr, nmean, nrstd);
         Acc sa = 0, sc = 0;
 #pragma unroll
         for (int i = 0; i < V; i++) {
             const uint32_t c = (uint32_t)(t + i * T) * N;
-            load_row<E, Acc, N>(xr, c, a.cols, h[i]);
-            load_row<E, Acc, N>(dr, c, a.cols, d[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-            const uint32_t c = (uint32_t)(t + i * T) * N;
+            renew(x[i]);
+            if (EVEN && c >= a.cols) continue;
             Acc g[N];
-            load_param<E, Acc, N>(a.gamma, a.wide, (Acc)1, c, a.cols, g);
+            load_param<E, Acc, N, EVEN>(a.gamma, a.wide, (Acc)1, c, a.cols, g);
 #pragma unroll
             for (int e = 0; e < N; e++) {
-                h[i][e] = c + e < a.cols ? (h[i][e] - mean) * rstd : (Acc)0;
-                sg[i][e] = fma_of(d[i][e], h[i][e], sg[i][e]);
-                sb[i][e] += d[i][e];
-                const Acc tt = d[i][e] * g[e];
+                const Acc dy = wide_of<E>(d[i], e);
+                const Acc h = c + (EVEN ? 0 : e) < a.cols ? (wide_of<E>(x[i], e) - mean) * rstd : (Acc)0;
+                sg[i][e] = fma_of(dy, h, sg[i][e]);
+                sb[i][e] += dy;
+                const Acc tt = dy * g[e];
                 sa += tt;
-                sc = fma_of(tt, h[i][e], sc);
-                d[i][e] = tt;
+                sc = fma_of(tt, h, sc);
             }
         }
-        if (!a.dx) continue;
-        sa = wave_sum(sa);
-        sc = wave_sum(sc);
-        if constexpr (T > 64) {
-            if ((threadIdx.x & 63) == 0) { scratch[turn][0][threadIdx.x >> 6] = sa; scratch[turn][1][threadIdx.x >> 6] = sc; }
-            __syncthreads();
-            sa = scratch[turn][0][0];
-            sc = scratch[turn][1][0];
+        if (a.dx) {
+            sa = wave_sum(sa);
+            sc = wave_sum(sc);
+            if constexpr (T > 64) {
+                if ((threadIdx.x & 63) == 0) { scratch[turn][0][threadIdx.x >> 6] = sa; scratch[turn][1][threadIdx.x >> 6] = sc; }
+                __syncthreads();
+                sa = scratch[turn][0][0];
+                sc = scratch[turn][1][0];
 #pragma unroll
-            for (int w = 1; w < W; w++) { sa += scratch[turn][0][w]; sc += scratch[turn][1][w]; }
+                for (int w = 1; w < W; w++) { sa += scratch[turn][0][w]; sc += scratch[turn][1][w]; }
+            }
+            sa *= inv_n;
+            sc *= inv_n;
+            E* xo = (E*)a.dx + row * a.ld_dx;
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const uint32_t c = (uint32_t)(t + i * T) * N;
+                renew(x[i]);
+                renew(d[i]);
+                if (c >= a.cols) continue;
+                Acc g[N], o[N];
+                load_param<E, Acc, N, EVEN>(a.gamma, a.wide, (Acc)1, c, a.cols, g);
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    const Acc h = (wide_of<E>(x[i], e) - mean) * rstd;
+                    o[e] = fma_of(rstd, wide_of<E>(d[i], e) * g[e] - fma_of(h, sc, sa), a.res ? wide_of<E>(r[i], e) : (Acc)0);
+                }
+                store_vec<E, Acc, EVEN>(xo, c, a.cols, o);
+            }
         }
-        sa *= inv_n;
-        sc *= inv_n;
-        E* xo = (E*)a.dx + row * a.ld_dx;
-        const E* rr = a.res ? (const E*)a.res + row * a.ld_res : nullptr;
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-            const uint32_t c = (uint32_t)(t + i * T) * N;
-            if (c >= a.cols) continue;
-            Acc r[N];
-            if (rr) load_row<E, Acc, N>(rr, c, a.cols, r);
-            else
-#pragma unroll
-                for (int e = 0; e < N; e++) r[e] = 0;
-#pragma unroll
-            for (int e = 0; e < N; e++) d[i][e] = fma_of(rstd, d[i][e] - fma_of(h[i][e], sc, sa), r[e]);
-            store_row<E, Acc, N>(xo, c, a.cols, d[i]);
-        }
+        for (int i = 0; i < V; i++) { x[i] = nx[i]; d[i] = nd[i]; if (a.res) r[i] = nr[i]; }
+        mean = nmean;
+        rstd = nrstd;
     }
     if (!a.part) return;
     Acc* pg = (Acc*)a.part + (uint64_t)blockIdx.x * 2 * a.cols;
     if constexpr (PER == 1) {
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            const uint32_t c = (uint32_t)(t + i * T) * N;
+            const uint32_t c = (uint32_t)(t0 + i * T) * N;
             store_row<Acc, Acc, N>(pg, c, a.cols, sg[i]);
             store_row<Acc, Acc, N>(pg + a.cols, c, a.cols, sb[i]);
         }
@@ -243,7 +320,7 @@ void norm_back_kernel(NormBackArgs a) {
 #pragma unroll
             for (int i = 0; i < V; i++)
 #pragma unroll
-                for (int e = 0; e < N; e++) join[threadIdx.x / T][(t + i * T) * N + e] = which ? sb[i][e] : sg[i][e];
+                for (int e = 0; e < N; e++) join[threadIdx.x / T][(t0 + i * T) * N + e] = which ? sb[i][e] : sg[i][e];
             __syncthreads();
             for (uint32_t c = threadIdx.x; c < a.cols; c += 256) {
                 Acc s = join[0][c];
@@ -400,17 +477,23 @@ int check_norm(const HipLayerNormArgs* u, NormArgs* a) {
 template <int DT, int T, int V>
 void launch_norm(const NormArgs& a, hipStream_t st) {
     constexpr int PER = T < 256 ? 256 / T : 1;
-    const uint64_t most = (uint64_t)eshkol_hip_num_cus() * (T > 256 ? 4 : 16);
+    const uint64_t most = (uint64_t)eshkol_hip_num_cus() * (T > 256 ? 2 : V >= 8 ? 4 : 8);
     const uint64_t grid = std::min<uint64_t>((a.rows + PER - 1) / PER, most);
-    hipLaunchKernelGGL((norm_kernel<DT, T, V>), dim3((unsigned)grid), dim3(T < 256 ? 256 : T), 0, st, a);
+    const dim3 g((unsigned)grid), b(T < 256 ? 256 : T);
+    if (a.cols % Vec16<typename Elem<DT>::T>::N == 0) hipLaunchKernelGGL((norm_kernel<DT, T, V, true>), g, b, 0, st, a);
+    else hipLaunchKernelGGL((norm_kernel<DT, T, V, false>), g, b, 0, st, a);
 }
 
 template <int DT>
 void dispatch_norm(const NormArgs& a, hipStream_t st) {
     const uint64_t nv = vectors(a.cols, DT);
+    /* a row per wave as long as it fits and there are rows enough to fill the device with waves */
+    const bool many = a.rows >= 4 * (uint64_t)eshkol_hip_num_cus();
     if (nv <= 64) launch_norm<DT, 64, 1>(a, st);
     else if (nv <= 128) launch_norm<DT, 64, 2>(a, st);
-    else if (nv <= 256) launch_norm<DT, 64, 4>(a, st);
+    else if (many && nv <= 256) launch_norm<DT, 64, 4>(a, st);
+    else if (many && nv <= 512) launch_norm<DT, 64, 8>(a, st);
+    else if (nv <= 256) launch_norm<DT, 256, 1>(a, st);
     else if (nv <= 512) launch_norm<DT, 256, 2>(a, st);
     else if (nv <= 1024) launch_norm<DT, 256, 4>(a, st);
     else if (nv <= 2048) launch_norm<DT, 256, 8>(a, st);
@@ -433,15 +516,17 @@ struct NormBackPlan {
 NormBackPlan plan_back(uint64_t rows, uint64_t cols, int dtype, bool want_params) {
     NormBackPlan p;
     const uint64_t nv = vectors(cols, dtype), acc = dtype == 0 ? 8 : 4;
-    p.threads = nv <= 128 ? 64 : nv <= 1024 ? 256 : nv <= 4096 ? 1024 : 0;
+    /* a row per wave while the sums of its columns (twice V vectors, widened) leave registers for three waves */
+    p.threads = nv <= (dtype >= 2 ? 128 : 256) ? 64 : nv <= 1024 ? 256 : nv <= 2048 ? 1024 : 0;
     p.per = p.threads == 64 ? 4 : 1;
     const uint64_t cus = (uint64_t)eshkol_hip_num_cus();
-    uint64_t most = p.threads == 1024 ? cus : 2 * cus;
+    uint64_t most = p.threads == 1024 ? cus : 4 * cus;
     if (p.threads == 0) {
         const uint64_t tiles = (nv + 255) / 256;
         most = std::max<uint64_t>(1, (8 * cus + tiles - 1) / tiles);
     }
-    p.grid = std::min<uint64_t>((rows + p.per - 1) / p.per, most);
+    /* two rows at least for every thread's sums, so that the second launch has less to add up than the first to read */
+    p.grid = std::min<uint64_t>((rows + 2 * p.per - 1) / (2 * p.per), most);
     p.sums_bytes = p.threads == 0 ? round_up_sz((size_t)(rows * 2 * acc), 256) : 0;
     p.part_bytes = want_params ? p.grid * 2 * cols * acc : 0;
     return p;
@@ -473,7 +558,9 @@ int check_back(const char* name, const HipLayerNormBackwardArgs* u, NormBackArgs
 
 template <int DT, int T, int V>
 void launch_back(const NormBackArgs& a, uint64_t grid, hipStream_t st) {
-    hipLaunchKernelGGL((norm_back_kernel<DT, T, V>), dim3((unsigned)grid), dim3(T < 256 ? 256 : T), 0, st, a);
+    const dim3 g((unsigned)grid), b(T < 256 ? 256 : T);
+    if (a.cols % Vec16<typename Elem<DT>::T>::N == 0) hipLaunchKernelGGL((norm_back_kernel<DT, T, V, true>), g, b, 0, st, a);
+    else hipLaunchKernelGGL((norm_back_kernel<DT, T, V, false>), g, b, 0, st, a);
 }
 
 template <int DT>
@@ -487,11 +574,13 @@ void dispatch_back(const NormBackArgs& a, const NormBackPlan& p, void* sums, voi
             hipLaunchKernelGGL((norm_back_long_kernel<DT>), dim3((unsigned)p.grid, (unsigned)((nv + 255) / 256)), dim3(256), 0, st, a, (const Acc*)sums);
         } else if (nv <= 64) launch_back<DT, 64, 1>(a, p.grid, st);
         else if (nv <= 128) launch_back<DT, 64, 2>(a, p.grid, st);
-        else if (nv <= 256) launch_back<DT, 256, 1>(a, p.grid, st);
+        else if (nv <= 256) {
+            if constexpr (DT >= 2) launch_back<DT, 256, 1>(a, p.grid, st);
+            else launch_back<DT, 64, 4>(a, p.grid, st);
+        }
         else if (nv <= 512) launch_back<DT, 256, 2>(a, p.grid, st);
         else if (nv <= 1024) launch_back<DT, 256, 4>(a, p.grid, st);
-        else if (nv <= 2048) launch_back<DT, 1024, 2>(a, p.grid, st);
-        else launch_back<DT, 1024, 4>(a, p.grid, st);
+        else launch_back<DT, 1024, 2>(a, p.grid, st);
     }
     if (gg || gb)
         hipLaunchKernelGGL((norm_join_kernel<Acc>), dim3((unsigned)((a.cols + 31) / 32), 2), dim3(256), 0, st,

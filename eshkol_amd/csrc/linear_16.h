@@ -189,7 +189,7 @@ __device__ __forceinline__ void finish_tile(const LinearArgs& g, v16f_t (&acc)[T
             const uint32_t row = row0 + t * 32 + r;
             if (row >= rows_end || c >= g.N) continue;
             float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            if (whole) finish_row8<BF16>(g.e, y_at, row, c, g.N, v, bias);
+            if (whole) finish_row8<BF16, true>(g.e, y_at, row, c, g.N, v, bias);
             else store_row<float, float, 8>(g.part + ((uint64_t)split * g.M + row) * g.part_ld, c, g.part_ld, v);
         }
     }

@@ -231,14 +231,15 @@ __device__ __forceinline__ void load_bias(const LinearEpilogue& e, uint32_t expe
 }
 
 /* z = v + bias, pre = z, y = act(z) + residual for columns c .. c + 7 of a row; y_at is the output matrix's
- * first element (its expert's, where C is one per expert) */
-template <bool BF16>
+ * first element (its expert's, where C is one per expert). STREAM: stores that do not displace what the L2 holds (the
+ * operands other tiles are about to read): 113 -> 104 us for an expert layer's two gradients, 8191 x 1024 x 2048 */
+template <bool BF16, bool STREAM = false>
 __device__ __forceinline__ void finish_row8(const LinearEpilogue& e, void* y_at, uint64_t row, uint32_t c, uint32_t N,
                                             float (&v)[8], const float (&bias)[8]) {
     typedef typename Half16<BF16>::T E;
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] += bias[i];
-    if (e.pre) store_row<E, float, 8>((E*)e.pre + row * e.ld_pre, c, N, v);
+    if (e.pre) store_row<E, float, 8, STREAM>((E*)e.pre + row * e.ld_pre, c, N, v);
     act8(v, e.act);
     if (e.residual) {
         float r[8];
@@ -246,8 +247,8 @@ __device__ __forceinline__ void finish_row8(const LinearEpilogue& e, void* y_at,
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] += r[i];
     }
-    if (e.out32) store_row<float, float, 8>((float*)y_at + row * e.ldy, c, N, v);
-    else store_row<E, float, 8>((E*)y_at + row * e.ldy, c, N, v);
+    if (e.out32) store_row<float, float, 8, STREAM>((float*)y_at + row * e.ldy, c, N, v);
+    else store_row<E, float, 8, STREAM>((E*)y_at + row * e.ldy, c, N, v);
 }
 
 }  // namespace linear
