@@ -259,7 +259,8 @@ __device__ __forceinline__ bool find_expert(const LinearArgs& g, uint32_t wg, ui
  * step's LDS reads and the requests between them, in an order the compiler is not to change. The one barrier of a block
  * stands before its last step: behind it every wave holds that step's fragments, so the block's LDS is free for block
  * + S, and the next block, whose first fragments the last step reads, has landed. */
-template <int BM_, int BN_, int BK_, int WM_, int WN_, int S_> struct TileShape {
+template <int BM_, int BN_, int BK_, int WM_, int WN_, int S_, bool GROUPS_ = false> struct TileShape {
+    static constexpr bool GROUPS = GROUPS_;
     static constexpr int BM = BM_, BN = BN_, BK = BK_, WM = WM_, WN = WN_, S = S_;
     static constexpr int THREADS = WM * WN * 64;
     static constexpr int SMEM = S * (BM + BN) * BK * 2 > WM * WN * park_bytes<BM / WM / 32, BN / WN / 32>()
@@ -424,14 +425,26 @@ void linear_tile_kernel(LinearArgs g) {
  * the other's last tiles, and two that would each leave CUs idle fill them together. */
 struct LinearPair {
     LinearArgs x, w;
-    uint32_t first;
+    uint32_t first, both;       /* workgroups of x, of x and w; the rest add up the bias gradient */
+    BiasJoin bias;
 };
+/* a column of an expert: the bias gradient's parts, in ascending order */
+__device__ __forceinline__ void join_bias(const BiasJoin& a, uint64_t id) {
+    const uint32_t expert = (uint32_t)(id / a.N), c = (uint32_t)(id % a.N);
+    if (expert >= a.experts) return;
+    const float* p = a.part + (uint64_t)expert * a.parts * a.N + c;
+    float s = 0.0f;
+#pragma unroll 16
+    for (uint32_t k = 0; k < a.parts; k++) s += p[(uint64_t)k * a.N];
+    a.out[(uint64_t)expert * a.N + c] = s;
+}
 template <int FB, class C, bool BF16, bool GROUPED>
 __global__ __launch_bounds__(C::THREADS)
 void linear_pair_kernel(LinearPair p) {
     extern __shared__ __align__(16) int8_t smem_l[];
     if (blockIdx.x < p.first) multiply_tile<ROWS_K, FB, C, BF16, GROUPED ? GROUP_ROWS : GROUP_NONE>(p.x, blockIdx.x, smem_l);
-    else multiply_tile<K_ROWS, K_ROWS, C, BF16, GROUPED ? GROUP_K : GROUP_NONE>(p.w, blockIdx.x - p.first, smem_l);
+    else if (blockIdx.x < p.both) multiply_tile<K_ROWS, K_ROWS, C, BF16, GROUPED ? GROUP_K : GROUP_NONE>(p.w, blockIdx.x - p.first, smem_l);
+    else join_bias(p.bias, (uint64_t)(blockIdx.x - p.both) * C::THREADS + threadIdx.x);
 }
 
 /* ---- a few rows: B streamed once, from memory into the matrix cores ---------------------------------------------
@@ -448,10 +461,11 @@ __device__ __forceinline__ v4f_t mfma16(const v4i_t& first, const v4i_t& second,
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h_t, first), __builtin_bit_cast(v8h_t, second), acc, 0, 0, 0);
 }
 
-/* eight 16-bit elements c .. c + 7 of a row of n, zeros beyond its end, as four words */
+/* eight 16-bit elements c .. c + 7 of a row of n, zeros beyond its end, as four words; THERE: all of them are */
+template <bool THERE = false>
 __device__ __forceinline__ v4i_t load8(const uint16_t* row, uint32_t c, uint32_t n) {
     typedef int v4iu_t __attribute__((ext_vector_type(4), aligned(2)));
-    if (c + 8 <= n) return *(const v4iu_t*)(row + c);
+    if (THERE || c + 8 <= n) return *(const v4iu_t*)(row + c);
     v4i_t v;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -535,6 +549,119 @@ void linear_thin_kernel(LinearArgs g) {
     }
 }
 
+/* ---- a few rows, K whole in a workgroup: no parts, no second launch ------------------------------------------------
+ * Sixteen waves share K and join in LDS; a workgroup's columns are few, so that there are workgroups enough.
+ *
+ * k contiguous (W [N][K]), up to sixteen rows: 16 columns, a wave takes every sixteenth 64 k. One row, K = N = 4096, bf16:
+ * 7.2 us, the kernel above 6.6 and its second launch 4. */
+template <bool BF16>
+__global__ __launch_bounds__(1024)
+void linear_few_rows_kernel(LinearArgs g) {
+    __shared__ __align__(16) v4f_t joined[16][64];
+    const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t n0 = blockIdx.x * 16;
+    const uint16_t* wr = g.b + (uint64_t)min(n0 + li, g.N - 1) * g.ldb;
+    const uint16_t* xr = g.a + (uint64_t)min((uint32_t)li, g.M - 1) * g.lda;
+    v4f_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto step = [&](uint32_t k0, auto full) {
+        constexpr bool FULL = decltype(full)::value != 0;       /* all 64 k are there */
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t k = k0 + 32 * h + 8 * lg;
+            acc = mfma16<BF16>(load8<FULL>(wr, k, g.K), load8<FULL>(xr, k, g.K), acc);
+        }
+    };
+    uint32_t k0 = 64 * wave;
+    for (; k0 + 1088 <= g.K; k0 += 2048) { step(k0, IC<1>{}); step(k0 + 1024, IC<1>{}); }
+    if (k0 + 64 <= g.K) { step(k0, IC<1>{}); k0 += 1024; }
+    if (k0 < g.K) step(k0, IC<0>{});
+    /* lane: row lane % 16, columns 4 (lane / 16) + 0..3; then a thread takes eight columns of a row, two lanes' four, over
+     * the waves in ascending order */
+    joined[wave][lane] = acc;
+    __syncthreads();
+    const uint32_t row = threadIdx.x & 15, pair = threadIdx.x >> 4, col = n0 + 8 * pair;
+    if (threadIdx.x >= 32 || row >= g.M || col >= g.N) return;
+    v4f_t lo = joined[0][32 * pair + row], hi = joined[0][32 * pair + 16 + row];
+#pragma unroll 5
+    for (int w = 1; w < 16; w++) { lo += joined[w][32 * pair + row]; hi += joined[w][32 * pair + 16 + row]; }
+    float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}, bias[8];
+    load_bias<BF16>(g.e, 0, col, g.N, bias);
+    finish_row8<BF16>(g.e, g.e.y, row, col, g.N, v, bias);
+}
+
+/* Columns contiguous (W [K][N]), up to four rows: 32 columns (one row, K = N = 4096, bf16: 7.7 us, the kernel above 5.0 and
+ * its second launch 4). A lane holds 8 k of 8 columns (transposed in its registers
+ * as above), and of a wave's 128 k lane l holds the sixteenth l / 4. The MFMA wants one k for all of its sixteen positions,
+ * so four of them, q = l / 4 % 4, carry the same columns at different k, and the other operand's sixteen positions are four
+ * rows at each of those four k: the blocks where the two q agree are the sums, the others are not looked at. */
+template <bool BF16>
+__global__ __launch_bounds__(1024)
+void linear_few_rows_strip_kernel(LinearArgs g) {
+    __shared__ __align__(16) float joined[64][4][33];           /* [wave, q][row][column] */
+    __shared__ float part[8][4][33];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    /* the two halves of a 128-byte line of W go to workgroups of one XCD, so that its L2 fetches the line once */
+    const uint32_t strip = ((blockIdx.x >> 4) * 8 + (blockIdx.x & 7)) * 2 + ((blockIdx.x >> 3) & 1);
+    const uint32_t n0 = strip * 32, c = n0 + 8 * (lane & 3);
+    if (n0 >= g.N) return;
+    v4f_t acc[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) acc[i] = (v4f_t){0.0f, 0.0f, 0.0f, 0.0f};
+    const int q = (lane >> 2) & 3;
+    auto step = [&](uint32_t k0, auto full) {
+        constexpr bool FULL = decltype(full)::value != 0;       /* all 128 k and 32 columns are there */
+        const uint32_t k = k0 + 8 * (lane >> 2);                /* of the columns' operand */
+        v4i_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) w[j] = FULL || k + j < g.K ? load8<FULL>(g.b + (uint64_t)(k + j) * g.ldb, c, g.N) : (v4i_t){0, 0, 0, 0};
+        /* of the rows' operand: position 4 q + row at k group 4 (lane / 16) + q: the same k */
+        const v4i_t x = load8<FULL>(g.a + (uint64_t)min((uint32_t)(lane & 3), g.M - 1) * g.lda, k, g.K);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            v4i_t f;
+#pragma unroll
+            for (int p = 0; p < 4; p++)
+                f[p] = (int)__builtin_amdgcn_perm((uint32_t)w[2 * p + 1][i / 2], (uint32_t)w[2 * p][i / 2], (i & 1) ? 0x07060302u : 0x05040100u);
+            acc[i] = mfma16<BF16>(f, x, acc[i]);
+        }
+    };
+    uint32_t k0 = 128 * wave;
+    if (n0 + 32 <= g.N) {
+        for (; k0 + 2176 <= g.K; k0 += 4096) { step(k0, IC<1>{}); step(k0 + 2048, IC<1>{}); }
+        if (k0 + 128 <= g.K) { step(k0, IC<1>{}); k0 += 2048; }
+    }
+    for (; k0 < g.K; k0 += 2048) step(k0, IC<0>{});
+    /* lane: position 4 q + row of the rows' operand, positions 4 (lane / 16) + r, column group r, of the columns' */
+    if (q == lane >> 4)
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) joined[wave * 4 + q][lane & 3][8 * r + i] = acc[i][r];
+    __syncthreads();
+    {
+        const int o = threadIdx.x & 127, p = threadIdx.x >> 7;
+        float s = joined[8 * p][o >> 5][o & 31];
+#pragma unroll
+        for (int k = 1; k < 8; k++) s += joined[8 * p + k][o >> 5][o & 31];
+        part[p][o >> 5][o & 31] = s;
+    }
+    __syncthreads();
+    const int row = threadIdx.x >> 2, group = threadIdx.x & 3;
+    const uint32_t col = n0 + 8 * group;
+    if (threadIdx.x >= 16 || (uint32_t)row >= g.M || col >= g.N) return;
+    float v[8], bias[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        v[i] = part[0][row][8 * group + i];
+#pragma unroll
+        for (int p = 1; p < 8; p++) v[i] += part[p][row][8 * group + i];
+    }
+    load_bias<BF16>(g.e, 0, col, g.N, bias);
+    finish_row8<BF16>(g.e, g.e.y, row, col, g.N, v, bias);
+}
+
 /* ---- around the products ---------------------------------------------------------------------------------------- */
 
 /* The parts of k added in ascending order, and the epilogue: a thread takes eight columns of a row. */
@@ -571,16 +698,6 @@ __device__ __forceinline__ void join_parts(const LinearArgs& g, uint32_t block) 
     finish_row8<BF16>(g.e, g.e.y, row, c, g.N, v, bias);
 }
 
-__device__ __forceinline__ void join_bias(const BiasJoin& a, uint32_t block) {
-    const uint64_t id = (uint64_t)block * 256 + threadIdx.x;
-    const uint32_t expert = (uint32_t)(id / a.N), c = (uint32_t)(id % a.N);
-    if (expert >= a.experts) return;
-    const float* p = a.part + (uint64_t)expert * a.parts * a.N + c;
-    float s = 0.0f;
-#pragma unroll 16
-    for (uint32_t k = 0; k < a.parts; k++) s += p[(uint64_t)k * a.N];
-    a.out[(uint64_t)expert * a.N + c] = s;
-}
 
 /* What is left to add up behind the products, in one launch: the parts of up to two products and of a bias gradient. */
 struct JoinArgs {
@@ -595,7 +712,7 @@ void linear_join_kernel(JoinArgs a) {
     if (b < a.blocks[0]) { join_parts<BF16, GROUPED>(a.product[0], b); return; }
     b -= a.blocks[0];
     if (b < a.blocks[1]) { join_parts<BF16, false>(a.product[1], b); return; }
-    join_bias(a.bias, b - a.blocks[1]);
+    join_bias(a.bias, (uint64_t)(b - a.blocks[1]) * 256 + threadIdx.x);
 }
 
 __device__ __forceinline__ void align_rows(const AlignArgs& a, uint32_t block) {
@@ -686,8 +803,12 @@ inline bool lds_ready(const void* kern, int bytes) {
 }
 
 typedef TileShape<256, 256, 64, 2, 4, 2> LargeTile;
-typedef TileShape<128, 256, 32, 2, 4, 3> WideTile;
-typedef TileShape<128, 128, 32, 2, 2, 3> SquareTile;
+typedef TileShape<128, 256, 32, 2, 4, 3, true> WideTile;
+typedef TileShape<128, 128, 32, 2, 2, 3, true> SquareTile;
+typedef TileShape<32, 128, 64, 1, 4, 3, true> Rows32Tile;
+typedef TileShape<64, 128, 64, 2, 2, 4, true> Rows64Tile;
+typedef TileShape<128, 256, 64, 2, 4, 3> WideAloneTile;
+typedef TileShape<128, 128, 64, 2, 2, 4> SquareAloneTile;
 
 
 /* the copy's work; the matrix is the copy from here on */
@@ -738,11 +859,11 @@ int launch_tile(Product* q, hipStream_t st) {
     hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(C::THREADS), C::SMEM, st, q->g);
     return 0;
 }
-/* the large tile is for products of one matrix (plan_products): a group's last rows would leave too much of it empty */
+/* the tiles that plan_products gives to products of one matrix alone have no kernels for groups */
 template <class C, bool BF16>
 int launch_tiles(Product* q, hipStream_t st) {
     const Shape& s = q->s;
-    if constexpr (C::BM < 256) {
+    if constexpr (C::GROUPS) {
         if (s.group == GROUP_K) return launch_tile<K_ROWS, K_ROWS, C, BF16, GROUP_K>(q, st);
         if (s.group == GROUP_ROWS) return s.fb == ROWS_K ? launch_tile<ROWS_K, ROWS_K, C, BF16, GROUP_ROWS>(q, st) : launch_tile<ROWS_K, K_ROWS, C, BF16, GROUP_ROWS>(q, st);
     }
@@ -751,34 +872,75 @@ int launch_tiles(Product* q, hipStream_t st) {
     return s.fb == ROWS_K ? launch_tile<ROWS_K, ROWS_K, C, BF16, GROUP_NONE>(q, st) : launch_tile<ROWS_K, K_ROWS, C, BF16, GROUP_NONE>(q, st);
 }
 template <int FB, class C, bool BF16, bool GROUPED>
-int launch_pair(Product* x, Product* w, hipStream_t st) {
+int launch_pair(Product* x, Product* w, const BiasJoin& bias, hipStream_t st) {
     auto kern = linear_pair_kernel<FB, C, BF16, GROUPED>;
     if (!lds_ready((const void*)kern, C::SMEM)) return -1;
     LinearPair p;
     const uint64_t a = fill_tiles<C>(x), b = fill_tiles<C>(w);
-    if (a + b > 0x7fffffffULL) return -1;
+    const uint64_t c = bias.out ? ((uint64_t)bias.N * bias.experts + C::THREADS - 1) / C::THREADS : 0;
+    if (a + b + c > 0x7fffffffULL) return -1;
     p.x = x->g;
     p.w = w->g;
     p.first = (uint32_t)a;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(a + b)), dim3(C::THREADS), C::SMEM, st, p);
+    p.both = (uint32_t)(a + b);
+    p.bias = bias;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(a + b + c)), dim3(C::THREADS), C::SMEM, st, p);
     return 0;
 }
 template <class C, bool BF16>
-int launch_pairs(Product* x, Product* w, hipStream_t st) {
+int launch_pairs(Product* x, Product* w, const BiasJoin& bias, hipStream_t st) {
     const bool rows_k = x->s.fb == ROWS_K;
     if (x->s.group == GROUP_ROWS) {
-        if constexpr (C::BM < 256) return rows_k ? launch_pair<ROWS_K, C, BF16, true>(x, w, st) : launch_pair<K_ROWS, C, BF16, true>(x, w, st);
+        if constexpr (C::GROUPS) return rows_k ? launch_pair<ROWS_K, C, BF16, true>(x, w, bias, st) : launch_pair<K_ROWS, C, BF16, true>(x, w, bias, st);
         else return -1;
     }
-    return rows_k ? launch_pair<ROWS_K, C, BF16, false>(x, w, st) : launch_pair<K_ROWS, C, BF16, false>(x, w, st);
+    return rows_k ? launch_pair<ROWS_K, C, BF16, false>(x, w, bias, st) : launch_pair<K_ROWS, C, BF16, false>(x, w, bias, st);
+}
+template <bool BF16>
+int launch_pairs(int tile, Product* x, Product* w, const BiasJoin& bias, hipStream_t st) {
+    switch (tile) {
+    case TILE_LARGE: return launch_pairs<LargeTile, BF16>(x, w, bias, st);
+    case TILE_WIDE: return launch_pairs<WideTile, BF16>(x, w, bias, st);
+    case TILE_WIDE_ALONE: return launch_pairs<WideAloneTile, BF16>(x, w, bias, st);
+    case TILE_SQUARE_ALONE: return launch_pairs<SquareAloneTile, BF16>(x, w, bias, st);
+    default: return launch_pairs<SquareTile, BF16>(x, w, bias, st);
+    }
+}
+/* tiles of 32 or 64 rows are for products whose first operand has k contiguous */
+template <class C, bool BF16>
+int launch_rows(Product* q, hipStream_t st) {
+    const bool rows_k = q->s.fb == ROWS_K;
+    if (q->s.fa != ROWS_K) return -1;
+    if (q->s.group == GROUP_ROWS) return rows_k ? launch_tile<ROWS_K, ROWS_K, C, BF16, GROUP_ROWS>(q, st) : launch_tile<ROWS_K, K_ROWS, C, BF16, GROUP_ROWS>(q, st);
+    return rows_k ? launch_tile<ROWS_K, ROWS_K, C, BF16, GROUP_NONE>(q, st) : launch_tile<ROWS_K, K_ROWS, C, BF16, GROUP_NONE>(q, st);
+}
+template <bool BF16>
+int launch_tiles(int tile, Product* q, hipStream_t st) {
+    if (q->kind == RUN_TILES_32) return launch_rows<Rows32Tile, BF16>(q, st);
+    if (q->kind == RUN_TILES_64) return launch_rows<Rows64Tile, BF16>(q, st);
+    switch (tile) {
+    case TILE_LARGE: return launch_tiles<LargeTile, BF16>(q, st);
+    case TILE_WIDE: return launch_tiles<WideTile, BF16>(q, st);
+    case TILE_WIDE_ALONE: return launch_tiles<WideAloneTile, BF16>(q, st);
+    case TILE_SQUARE_ALONE: return launch_tiles<SquareAloneTile, BF16>(q, st);
+    default: return launch_tiles<SquareTile, BF16>(q, st);
+    }
 }
 template <bool BF16>
 int launch_thin(Product* q, hipStream_t st) {
     const bool rows = q->s.group == GROUP_ROWS;
+    if (q->kind == RUN_STREAM_WHOLE) {
+        if (q->s.fb == K_ROWS) hipLaunchKernelGGL((linear_few_rows_strip_kernel<BF16>), dim3((tiles_of(q->s.N, 32) + 15) / 16 * 16), dim3(1024), 0, st, q->g);
+        else hipLaunchKernelGGL((linear_few_rows_kernel<BF16>), dim3(tiles_of(q->s.N, 16)), dim3(1024), 0, st, q->g);
+        return 0;
+    }
     const dim3 grid(tiles_of(q->s.N, 128), q->splits, rows ? q->g.experts : 1);
-#define THIN(FB, RT) do { if (rows) hipLaunchKernelGGL((linear_thin_kernel<FB, RT, BF16, true>), grid, dim3(256), 0, st, q->g); \
-                          else hipLaunchKernelGGL((linear_thin_kernel<FB, RT, BF16, false>), grid, dim3(256), 0, st, q->g); } while (0)
-    if (q->s.fb == ROWS_K) { if (q->rt == 1) THIN(ROWS_K, 1); else if (q->rt == 2) THIN(ROWS_K, 2); else THIN(ROWS_K, 4); }
+    /* more than sixteen rows by expert are tiles */
+#define THIN(FB, RT) hipLaunchKernelGGL((linear_thin_kernel<FB, RT, BF16, false>), grid, dim3(256), 0, st, q->g)
+    if (rows) {
+        if (q->s.fb == ROWS_K) hipLaunchKernelGGL((linear_thin_kernel<ROWS_K, 1, BF16, true>), grid, dim3(256), 0, st, q->g);
+        else hipLaunchKernelGGL((linear_thin_kernel<K_ROWS, 1, BF16, true>), grid, dim3(256), 0, st, q->g);
+    } else if (q->s.fb == ROWS_K) { if (q->rt == 1) THIN(ROWS_K, 1); else if (q->rt == 2) THIN(ROWS_K, 2); else THIN(ROWS_K, 4); }
     else { if (q->rt == 1) THIN(K_ROWS, 1); else if (q->rt == 2) THIN(K_ROWS, 2); else THIN(K_ROWS, 4); }
 #undef THIN
     return 0;
@@ -793,7 +955,7 @@ int run_products(Product* q, int n, int tile, const SlopeArgs* slope, const Bias
     if (slope) pre.slope = *slope;
     int copies = 0;
     for (int i = 0; i < n; i++) {
-        if (q[i].thin) continue;
+        if (q[i].streams()) continue;
         for (Matrix* m : {&q[i].a, &q[i].b}) {
             if (!m->copy) continue;
             const uint64_t bytes = m->copy_bytes;
@@ -812,14 +974,14 @@ int run_products(Product* q, int n, int tile, const SlopeArgs* slope, const Bias
         ws += q[i].part_bytes;
     }
     int rc = 0;
-    if (n == 2 && !q[0].thin && !q[1].thin)
-        rc = tile == TILE_LARGE ? launch_pairs<LargeTile, BF16>(&q[0], &q[1], st)
-             : tile == TILE_WIDE ? launch_pairs<WideTile, BF16>(&q[0], &q[1], st) : launch_pairs<SquareTile, BF16>(&q[0], &q[1], st);
-    else
-        for (int i = 0; i < n && !rc; i++)
-            rc = q[i].thin ? launch_thin<BF16>(&q[i], st)
-                 : tile == TILE_LARGE ? launch_tiles<LargeTile, BF16>(&q[i], st)
-                 : tile == TILE_WIDE ? launch_tiles<WideTile, BF16>(&q[i], st) : launch_tiles<SquareTile, BF16>(&q[i], st);
+    bool bias_done = !bias || !bias->out;
+    if (n == 2 && q[0].kind == RUN_TILES && q[1].kind == RUN_TILES) {
+        /* without parts to join there is no launch behind the products: the bias gradient is added up beside them */
+        const bool beside = !bias_done && q[0].splits <= 1 && q[1].splits <= 1;
+        rc = launch_pairs<BF16>(tile, &q[0], &q[1], beside ? *bias : BiasJoin{}, st);
+        bias_done |= beside;
+    } else
+        for (int i = 0; i < n && !rc; i++) rc = q[i].streams() ? launch_thin<BF16>(&q[i], st) : launch_tiles<BF16>(tile, &q[i], st);
     if (rc) return rc;
     bool grouped = false;
     for (int i = 0; i < n; i++) {
@@ -833,7 +995,7 @@ int run_products(Product* q, int n, int tile, const SlopeArgs* slope, const Bias
         joins += b;
         grouped |= q[i].s.group == GROUP_ROWS;
     }
-    if (bias && bias->out) {
+    if (!bias_done) {
         join.bias = *bias;
         const uint64_t b = ((uint64_t)bias->N * bias->experts + 255) / 256;
         if (b > 0x7fffffffULL) return -1;

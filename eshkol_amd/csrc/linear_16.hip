@@ -14,7 +14,10 @@ Matrix matrix_of(const void* p, uint64_t ld, uint64_t stride, uint64_t rows, uin
     if (m.copy) m.copy_bytes = round_up_sz((size_t)(count * rows * round_up_sz(cols, 8) * 2), 256);
     return m;
 }
-/* a product of a few rows, by the kernel that streams B: whole rows of tiles would be empty */
+/* How a product is run. Up to sixteen rows (on average, by expert) B is streamed past them, up to 64 in tiles of 32 or 64
+ * rows: the streaming kernel's loads of more rows outgrow those of B (K = N = 4096, W [N][K], bf16, us without the second
+ * launch: 32 rows 11.3 and 7.6, 64 rows 16.9 and 8.4; one row 6.6 and 7.6). The tiles want aligned operands, and a copy of
+ * B would cost more than they gain. */
 Product make_product(const Shape& s, const Matrix& a, const Matrix& b) {
     Product q = {};
     q.s = s;
@@ -22,11 +25,18 @@ Product make_product(const Shape& s, const Matrix& a, const Matrix& b) {
     q.b = b;
     q.splits = 1;
     q.part_k = (uint32_t)round_up_sz((size_t)s.K, 64);
-    q.thin = s.fa == ROWS_K && s.group != GROUP_K && (s.group == GROUP_ROWS ? s.M <= 16 * s.experts : s.M <= 64);
-    if (q.thin) {
-        const uint64_t rows = s.group == GROUP_ROWS ? (s.M + s.experts - 1) / s.experts : s.M;
-        q.rt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    }
+    q.kind = RUN_TILES;
+    if (s.fa != ROWS_K || s.group == GROUP_K) return q;
+    const bool grouped = s.group == GROUP_ROWS;
+    const uint64_t rows = grouped ? (s.M + s.experts - 1) / s.experts : s.M;
+    if (rows > 64) return q;
+    q.rt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    if (rows > 16 && !a.copy && !b.copy) { q.kind = rows <= 32 && !grouped ? RUN_TILES_32 : RUN_TILES_64; return q; }
+    if (rows > 16 && grouped) return q;
+    /* K whole in a workgroup where the narrow strips of columns alone give a third of the CUs work */
+    const uint64_t strips = tiles_of(s.N, s.fb == K_ROWS ? 32 : 16);
+    const bool whole = !grouped && s.M <= (s.fb == K_ROWS ? 4 : 16) && strips * 3 >= (uint64_t)eshkol_hip_num_cus();
+    q.kind = whole ? RUN_STREAM_WHOLE : RUN_STREAM;
     return q;
 }
 /* cuts K into about `want` parts of at least `least` */
@@ -34,7 +44,7 @@ void split_product(Product* q, uint64_t want, uint64_t least) {
     const uint64_t k64 = round_up_sz((size_t)q->s.K, 64);
     uint64_t splits = std::min<uint64_t>(want, k64 / least);
     if (splits <= 1) return;
-    const uint64_t part = round_up_sz((size_t)((k64 + splits - 1) / splits), q->thin ? 128 : 64);
+    const uint64_t part = round_up_sz((size_t)((k64 + splits - 1) / splits), q->kind == RUN_STREAM ? 128 : 64);
     splits = (q->s.K + part - 1) / part;
     if (splits <= 1) return;
     q->part_k = (uint32_t)part;
@@ -42,31 +52,45 @@ void split_product(Product* q, uint64_t want, uint64_t least) {
     q->part_ld = (uint32_t)round_up_sz((size_t)q->s.N, 8);
     q->part_bytes = round_up_sz((size_t)(splits * q->s.M * q->part_ld * 4), 256);
 }
-/* The tile of one or two products launched together, and how their K is cut. */
+/* The tile of one or two products launched together, and how their K is cut. Times are of bf16 products, us.
+ * 256 x 256 where at least three quarters of the CUs get one (8192^3: 819; 128 x 256 921, 128 x 128 1170), products of one
+ * matrix only: the last rows of a group leave half a tile empty on average.
+ * 128 x 256 where that many of those there are (the two products of 4096 x 1024 x 4096: 74, 128 x 128 79; 16384 rows of 64
+ * experts, 1024 x 4096: 236 and 279). Two fit on a CU; where no CU gets two, blocks of 64 k instead of 32 need half the
+ * barriers (the same two: 65).
+ * 128 x 128 otherwise, three on a CU, or alone with blocks of 64 k (4096 x 1024 x 4096: 41 and 47). */
 int plan_products(Product* q, int n) {
     const uint64_t cus = (uint64_t)eshkol_hip_num_cus();
-    uint64_t large = 0, wide = 0, square = 0;
-    bool any = false;
+    uint64_t large = 0, wide = 0, square = 0, work = 0;
+    bool any = false, grouped = false;
     for (int i = 0; i < n; i++) {
-        if (q[i].thin) {
-            const Shape& s = q[i].s;
+        const Shape& s = q[i].s;
+        if (q[i].kind != RUN_TILES) {
             const uint64_t have = (uint64_t)tiles_of(s.N, 128) * (s.group == GROUP_ROWS ? std::min(s.experts, s.M) : 1);
-            split_product(&q[i], (2 * cus + have - 1) / have, 128);
+            if (q[i].kind == RUN_STREAM) split_product(&q[i], (2 * cus + have - 1) / have, 128);
+            else if (q[i].kind != RUN_STREAM_WHOLE && s.group == GROUP_NONE) split_product(&q[i], (cus + have - 1) / have, 256);
             continue;
         }
         any = true;
-        large += tile_count(q[i].s, 256, 256);
-        wide += tile_count(q[i].s, 128, 256);
-        square += tile_count(q[i].s, 128, 128);
+        grouped |= s.group != GROUP_NONE;
+        large += tile_count(s, 256, 256);
+        wide += tile_count(s, 128, 256);
+        square += tile_count(s, 128, 128);
+        work += tile_count(s, 128, 128) * ((s.K + 63) / 64);
     }
     if (!any) return TILE_SQUARE;
-    bool grouped = false;
-    for (int i = 0; i < n; i++) grouped |= q[i].s.group != GROUP_NONE;
-    if (!grouped && large * 4 >= cus * 3) return TILE_LARGE;
-    if (wide * 4 >= cus * 3) return TILE_WIDE;
-    if (!grouped && square * 2 < cus)
-        for (int i = 0; i < n; i++) if (!q[i].thin) split_product(&q[i], cus / square, 512);
-    return TILE_SQUARE;
+    if (grouped) return wide * 4 >= cus * 3 ? TILE_WIDE : TILE_SQUARE;
+    if (large * 4 >= cus * 3) return TILE_LARGE;
+    if (wide * 4 >= cus * 3) return wide <= cus ? TILE_WIDE_ALONE : TILE_WIDE;
+    /* too few tiles for the CUs: K is cut so that every workgroup has about a CU's share of the blocks, at least 512 of K */
+    const uint64_t share = std::max<uint64_t>(1, work / cus);
+    uint64_t workgroups = 0;
+    for (int i = 0; i < n; i++) {
+        if (q[i].kind != RUN_TILES) continue;
+        if (square < cus) split_product(&q[i], ((q[i].s.K + 63) / 64 + share / 2) / share, 512);
+        workgroups += tile_count(q[i].s, 128, 128) * q[i].splits;
+    }
+    return workgroups <= cus + cus / 4 ? TILE_SQUARE_ALONE : TILE_SQUARE;
 }
 
 uint64_t products_bytes(const Product* q, int n) {
@@ -210,7 +234,7 @@ int plan_backward(const char* name, HipExpertsBackwardArgs u, bool grouped, Back
     const Matrix w = matrix_of(u.w, u.ldw, u.w_stride, wr, wc, experts), x = matrix_of(u.x, u.ldx, 0, u.rows, u.K, 1);
     Matrix dz = matrix_of(u.grad_y, u.ld_grad_y, 0, u.rows, u.N, 1);
     /* dz has room of its own where there is an activation, or where grad_y is not as the tiled kernel wants it */
-    const bool tiled = want_w || (want_x && !make_product(sx, dz, w).thin);
+    const bool tiled = want_w || (want_x && !make_product(sx, dz, w).streams());
     const bool make_dz = some && ((u.act && (want_x || want_w)) || (tiled && dz.copy));
     const uint64_t ld_dz = round_up_sz((size_t)u.N, 8);
     if (make_dz) dz = matrix_of((const void*)(uintptr_t)256, ld_dz, 0, u.rows, ld_dz, 1);       /* its address is known later */

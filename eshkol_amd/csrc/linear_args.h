@@ -86,17 +86,20 @@ struct Shape {
     int fa, fb, group;
     uint64_t M, N, K, experts;
 };
-enum { TILE_LARGE, TILE_WIDE, TILE_SQUARE };
+/* How a product is run: tiles of a shape that all of a launch share; tiles of 32 or 64 rows; B streamed past at most 64 rows
+ * (in parts of K that a second launch joins, or with K whole in a workgroup) */
+enum { RUN_TILES, RUN_TILES_32, RUN_TILES_64, RUN_STREAM, RUN_STREAM_WHOLE };
+enum { TILE_LARGE, TILE_WIDE, TILE_WIDE_ALONE, TILE_SQUARE, TILE_SQUARE_ALONE };
 
 struct Product {
     Shape s;
     Matrix a, b;
     LinearArgs g;
-    bool thin;
-    int rt;
+    int kind, rt;               /* rt: sixteens of rows of RUN_STREAM              */
     uint32_t splits, part_k, part_ld;
     uint64_t part_bytes;
-    uint64_t copy_bytes() const { return thin ? 0 : a.copy_bytes + b.copy_bytes; }
+    bool streams() const { return kind == RUN_STREAM || kind == RUN_STREAM_WHOLE; }     /* at any alignment */
+    uint64_t copy_bytes() const { return streams() ? 0 : a.copy_bytes + b.copy_bytes; }
 };
 
 inline uint32_t tiles_of(uint64_t n, uint32_t t) { return (uint32_t)((n + t - 1) / t); }

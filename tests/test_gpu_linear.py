@@ -181,6 +181,41 @@ def test_linear_backward(gpu, size, dtype, trans):
     t.check_backward(*t.backward(wtype), wtype)
 
 
+# K whole in a workgroup (1 to 4 rows, 16 with W [N][K]); tiles of 32 and of 64 rows, with k in parts
+FEW = [(1, 4096, 3000), (4, 1000, 2760), (3, 137, 4099), (2, 2304, 2731), (16, 520, 1400), (5, 4100, 1536), (11, 65, 1501), (20, 128, 3008), (32, 1096, 256),
+       (48, 2048, 136), (64, 264, 1416), (40, 72, 8)]
+
+
+@pytest.mark.parametrize("trans", [0, 1])
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=lambda t: NAMES[t])
+@pytest.mark.parametrize("size", FEW, ids=str)
+def test_few_rows(gpu, size, dtype, trans):
+    print("case: few rows", size, NAMES[dtype], trans, flush=True)
+    t = Layer(*size, dtype, trans, size[1] % 5, residual=True, seed=9)
+    t.check_forward(*t.forward())
+    t.check_backward(*t.backward(F32), F32)
+
+
+# products that take each of the tiles: 256 x 256; 128 x 256, one and two on a CU; 128 x 128, three on a CU and alone
+TILES = [(3600, 200, 3592), (2000, 136, 3000), (2816, 96, 3100), (2432, 104, 2400), (1000, 330, 1100)]
+
+
+@pytest.mark.parametrize("trans", [0, 1])
+@pytest.mark.parametrize("size", TILES, ids=str)
+def test_every_tile_forward(gpu, size, trans):
+    print("case: tiles forward", size, trans, flush=True)
+    t = Layer(*size, BF16 if trans else F16, trans, 4, residual=True)
+    t.check_forward(*t.forward())
+
+
+@pytest.mark.parametrize("trans", [0, 1])
+@pytest.mark.parametrize("size", [(2000, 3000, 1999), (1300, 2100, 1500), (2900, 1500, 1504), (1900, 1040, 1000), (900, 600, 1300)], ids=str)
+def test_every_tile_backward(gpu, size, trans):
+    print("case: tiles backward", size, trans, flush=True)
+    t = Layer(*size, F16 if trans else BF16, trans, 0 if trans else 1)
+    t.check_backward(*t.backward())
+
+
 @pytest.mark.parametrize("code", ACTS)
 @pytest.mark.parametrize("M", [20, 100])
 @pytest.mark.parametrize("param", [BF16, F32])
@@ -356,7 +391,9 @@ def test_experts_far_apart(gpu, M):
 # (rows, offsets): one expert; empty ones first, last, between; one row each; one with everything; more than 64 experts;
 # rows of no expert in front and behind; groups that end on, before and behind a tile's edge; many rows (the tiled kernel)
 GROUPS = [(5, [0, 5]), (6, [0, 0, 6, 6]), (3, [0, 1, 2, 3]), (40, [0, 0, 0, 40, 40]), (20, [3, 5, 5, 11]), (7, [0, 0, 0]), (200, list(range(0, 132, 2)) + [200]),
-          (300, [0, 128, 256, 300]), (500, [0, 127, 127, 256, 500]), (700, [10, 150, 151, 430, 600]), (1300, [0] * 20 + [600] * 30 + [1299])]
+          (300, [0, 128, 256, 300]), (500, [0, 127, 127, 256, 500]), (700, [10, 150, 151, 430, 600]), (1300, [0] * 20 + [600] * 30 + [1299]),
+          # enough tiles for the wide ones; 17 to 64 rows on average, aligned and not
+          (5001, list(range(0, 5001, 100)) + [5001]), (1301, list(range(0, 1301, 26)) + [1301]), (1302, list(range(0, 1302, 26)) + [1302])]
 
 
 @pytest.mark.parametrize("trans", [0, 1])
