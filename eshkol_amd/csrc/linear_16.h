@@ -1,18 +1,29 @@
 /*
- * The tiled 16-bit product behind the linear layer and the products by expert
- * (gpu_hip_layers.h): C[m][n] = sum_k A(m, k) B(n, k) with fp32 sums on the matrix
- * cores and the layer's epilogue, operands as the caller holds them.
+ * The kernels behind the linear layer and the products by expert (gpu_hip_layers.h):
+ * C[m][n] = sum_k A(m, k) B(n, k) of 16-bit operands as the caller holds them, with
+ * fp32 sums on the matrix cores and the layer's epilogue; what a backward pass needs
+ * before its two products and adds up behind them. Compiled once per element type.
  *
  * Forms. k contiguous in both (grad_x of a layer, and W held [N][K]), k contiguous
  * in A only (forward with W [K][N]), k contiguous in neither (grad_w). Operands go
  * from global memory straight into LDS, 16 bytes a lane (buffer_load ... lds), in
- * blocks of 64 k. An operand with k contiguous lies in LDS as rows of 128 bytes
- * and a fragment is one 16-byte read; one with its rows contiguous lies as 64 rows
- * of k, and ds_read_b64_tr_b16 hands every lane four k of its own row, so no
+ * blocks of 32 or 64 k. An operand with k contiguous lies in LDS as rows of 64 or
+ * 128 bytes and a fragment is one 16-byte read; one with its rows contiguous lies as
+ * rows of k, and ds_read_b64_tr_b16 hands every lane four k of its own row, so no
  * operand is ever transposed in memory. Both layouts are permuted inside a row
- * (16-byte chunks by row / 2 modulo 8, 32-byte units by k modulo 4) so that the
- * lanes served together fall into different banks; a load to LDS writes lanes in
- * order, so it is the global address that is permuted.
+ * (16-byte chunks by row / 2 modulo 8, or row / 4 modulo 4; 32-byte units by k modulo
+ * 4) so that the lanes served together fall into different banks; a load to LDS
+ * writes lanes in order, so it is the global address that is permuted. Measured: one
+ * LDS cycle in a hundred is a conflict, all of them the epilogue's.
+ *
+ * What bounds the tiles. 8192^3 with the 256 x 256 tile: 820-860 us (1.28-1.34
+ * PFLOP/s), the matrix pipe busy 67 per cent of the time; without its loads the loop
+ * takes 670 us, without its multiplications 680: operand blocks arrive in the L2 from
+ * behind it at the rate at which they are multiplied, and what is lost is where the
+ * two wait for each other. More blocks in flight (four and five of 32 k) gained
+ * nothing (880 us), and lines requested two blocks ahead into the L2 cost more
+ * request slots than they saved time (925). Smaller tiles are bound by the same
+ * stream sooner: about 55 GB/s per CU of operand blocks, whatever their shape.
  *
  * Edges. Addresses outside an operand are moved to ones inside it; what they bring
  * only reaches outputs that are not stored, except along k, where the fragments of
@@ -365,15 +376,17 @@ __device__ __forceinline__ void multiply_tile(const LinearArgs& g, uint32_t wg, 
             else a[W][I - TN] = fa.read(tile, KS, I - TN);
         };
         static_for<TM + TN>([&](auto i) { read(IC<0>{}, smem_l, IC<0>{}, i); });
-        /* one k-step: its multiplications with the reads of (tile, next step) between them, then mem(0 ..) */
+        /* one k-step: its multiplications, two reads of (tile, next step) behind each of the first of them (spread evenly
+         * over all of them 8192^3 took 866 us instead of 856), mem(i) behind the i-th */
         auto kstep = [&](auto which, const int8_t* tile, auto next, auto mem) {
             constexpr int W = decltype(which)::value;
             constexpr int MF = TM * TN, RD = TM + TN;
+            static_assert(RD <= 2 * MF, "every fragment has its multiplication");
             static_for<MF>([&](auto i) {
                 constexpr int I = decltype(i)::value, T = I / TN, U_ = I % TN;
                 mfma32<BF16>(b[W][U_], a[W][T], acc[T][U_]);
                 static_for<RD>([&](auto r) {
-                    if constexpr (decltype(r)::value * MF / RD == I) read(IC<1 - W>{}, tile, next, r);
+                    if constexpr (decltype(r)::value / 2 == I) read(IC<1 - W>{}, tile, next, r);
                 });
                 mem(i);
                 __builtin_amdgcn_sched_barrier(0);

@@ -130,6 +130,17 @@ int check_room(const char* name, const void* ws, uint64_t have, uint64_t need) {
     return -2;
 }
 
+/* a launch holds 2^31 - 1 workgroups; nothing is queued before this is known */
+int check_tiles(const char* name, const Product* q, int n) {
+    uint64_t total = 0;
+    for (int i = 0; i < n; i++) {
+        const uint64_t tiles = q[i].kind == RUN_TILES ? tile_count(q[i].s, 128, 128) : tile_count(q[i].s, 32, 128);
+        total += (tiles + 8) * q[i].splits;
+    }
+    if (total > 0x3fffffffULL) LAYER_REFUSE(name, "%llu tiles", (unsigned long long)total);
+    return 0;
+}
+
 /* ---- forward -------------------------------------------------------------------------------------------------------- */
 
 struct ForwardCall {
@@ -162,7 +173,7 @@ int plan_forward(const char* name, HipExpertsArgs u, const void* residual, uint6
     e.pre = (uint16_t*)u.pre; e.ld_pre = u.ld_pre;
     f->q.g.offsets = grouped ? u.offsets : nullptr;
     f->tile = plan_products(&f->q, 1);
-    return 0;
+    return check_tiles(name, &f->q, 1);
 }
 int64_t forward_workspace(const char* name, const HipExpertsArgs& u, const void* residual, uint64_t ld_res, bool grouped) {
     ForwardCall f;
@@ -272,7 +283,7 @@ int plan_backward(const char* name, HipExpertsBackwardArgs u, bool grouped, Back
         q.g.offsets = a.offsets;
     }
     c->tile = plan_products(c->q, c->n);
-    return 0;
+    return check_tiles(name, c->q, c->n);
 }
 uint64_t backward_bytes(const BackwardCall& c) { return c.dz_bytes + c.sum_bytes + products_bytes(c.q, c.n); }
 

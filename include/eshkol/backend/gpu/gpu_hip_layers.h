@@ -49,7 +49,7 @@ enum {
     HIP_ACT_RELU = 2,       /* derivative 0 at 0 */
     HIP_ACT_GELU = 3,       /* z Phi(z), Phi the normal distribution's integral (no tanh form) */
     HIP_ACT_SILU = 4        /* z / (1 + e^-z) */
-};
+};                          /* at an infinity: the limit (gelu and silu 0 at -infinity); NaN stays NaN */
 
 /* ---- layer norm --------------------------------------------------------------
  * y = (x - mean) rstd gamma + beta for every row of `cols` elements,

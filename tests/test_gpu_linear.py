@@ -51,9 +51,10 @@ class Layer:
     def groups(self):
         return [(0, self.M)] if self.offsets is None else list(zip(self.offsets[:-1], self.offsets[1:]))
 
-    def W(self, e):
-        w = self.w.values[e]
-        return w.T if self.trans else w
+    def W(self):
+        """The experts' matrices as [K][N] each."""
+        w = self.w.values
+        return w.transpose(0, 2, 1) if self.trans else w
 
     def out(self, shape, dtype=None):
         dtype = self.dtype if dtype is None else dtype
@@ -76,15 +77,17 @@ class Layer:
 
     def check_forward(self, y, z, note="", residual=None):
         got_y, got_z = y.get(), z.get() if z else None
+        every_x, every_w = self.x.values, self.W()
+        every_bias = self.bias.values.reshape(self.E, self.N) if self.bias else np.zeros((self.E, self.N))
+        every_r = None if self.residual is None else (self.residual.values if residual is None else residual)
         for e, (a, b) in enumerate(self.groups()):
-            X, W = self.x.values[a:b], self.W(e)
-            bias = self.bias.values.reshape(self.E, self.N)[e] if self.bias else np.zeros(self.N)
+            X, W, bias = every_x[a:b], every_w[e], every_bias[e]
             want = X @ W + bias
             err = 2 * (self.K + 8) * U * (np.abs(X) @ np.abs(W)) + 2 * U * (np.abs(want) + np.abs(bias))
             if z:
                 close(got_z[a:b], want, err * (1 + HALF[self.dtype]) + HALF[self.dtype] * np.abs(want) + FLOOR[self.dtype], note + " pre, expert %d" % e)
             f = act(want, self.code)
-            r = 0.0 if self.residual is None else (self.residual.values if residual is None else residual)[a:b]
+            r = 0.0 if every_r is None else every_r[a:b]
             err = 1.13 * err + act_error(want, self.code) * np.abs(f) + 2 * U * (np.abs(f) + np.abs(r))
             close(got_y[a:b], f + r, err * (1 + HALF[self.dtype]) + HALF[self.dtype] * np.abs(f + r) + FLOOR[self.dtype], note + " y, expert %d" % e)
         for m in (y, z):
@@ -133,8 +136,9 @@ class Layer:
         got_x = gx.get() if gx else None
         got_w = gw.get().reshape(self.w.shape) if gw else None
         got_b = gb.get() if gb else None
+        every_w = self.W()
         for e, (a, b) in enumerate(self.groups()):
-            W, d, x, c = self.W(e), DZ[a:b], X[a:b], cut[a:b]
+            W, d, x, c = every_w[e], DZ[a:b], X[a:b], cut[a:b]
             if gx:
                 want = d @ W.T
                 err = c @ np.abs(W.T) + 2 * (self.N + 8) * U * (np.abs(d) @ np.abs(W.T))
@@ -253,8 +257,7 @@ def test_activations_at_the_ends_of_the_range(gpu):
     z = np.array([np.inf, -np.inf, big, -big, np.nan, 200.0, -200.0, 14.0, -14.0])
     limits = {0: z, 1: np.array([1, -1, 1, -1, np.nan, 1, -1, 1, -1]), 2: np.array([np.inf, 0, big, 0, np.nan, 200, 0, 14, 0])}
     limits[3] = limits[4] = limits[2]
-    flat = {0: z * 0 + 1, 1: z * 0, 2: np.array([1, 0, 1, 0, np.nan, 1, 0, 1, 0])}
-    flat[0][:], flat[1][[0, 1, 2, 3]] = 1, 0
+    flat = {1: np.array([0, 0, 0, 0, np.nan, 0, 0, 0, 0]), 2: np.array([1, 0, 1, 0, np.nan, 1, 0, 1, 0])}
     flat[3] = flat[4] = flat[2]
     for code in ACTS:
         for M in (4, 70):
@@ -262,7 +265,9 @@ def test_activations_at_the_ends_of_the_range(gpu):
             t.x = Mat((M, 8), BF16, values=np.zeros((M, 8)))
             t.bias = vec(z[None], F32)
             y = t.forward()[0].get()
-            close(y, np.broadcast_to(limits[code], y.shape), 1.2e-5 + HALF[BF16] * np.abs(limits[code][np.isfinite(limits[code])]).max() * (np.abs(y) > 1e30), "act %d" % code)
+            # the bf16 nearest to 14 and 200 are exact; tanh(14) and Phi(14) are 1 to 12 digits, z Phi(z) at -14 is 1e-43
+            tol = 1e-11 + HALF[BF16] * np.nan_to_num(np.abs(limits[code]), nan=0, posinf=0) * (np.abs(z) > 1e30)
+            close(y, np.broadcast_to(limits[code], y.shape), np.broadcast_to(tol + (1.2e-5 if code == 4 else 0), y.shape), "act %d" % code)
         if code:
             t = Layer(1, 8, len(z), BF16, 0, code, F32)
             t.dy = Mat((1, len(z)), BF16, values=np.ones((1, len(z))))
@@ -392,6 +397,8 @@ def test_experts_far_apart(gpu, M):
 # rows of no expert in front and behind; groups that end on, before and behind a tile's edge; many rows (the tiled kernel)
 GROUPS = [(5, [0, 5]), (6, [0, 0, 6, 6]), (3, [0, 1, 2, 3]), (40, [0, 0, 0, 40, 40]), (20, [3, 5, 5, 11]), (7, [0, 0, 0]), (200, list(range(0, 132, 2)) + [200]),
           (300, [0, 128, 256, 300]), (500, [0, 127, 127, 256, 500]), (700, [10, 150, 151, 430, 600]), (1300, [0] * 20 + [600] * 30 + [1299]),
+          # a thousand experts, most of them without rows
+          (400, [0] * 500 + [3] * 200 + [200] * 200 + [399] * 101),
           # enough tiles for the wide ones; 17 to 64 rows on average, aligned and not
           (5001, list(range(0, 5001, 100)) + [5001]), (1301, list(range(0, 1301, 26)) + [1301]), (1302, list(range(0, 1302, 26)) + [1302])]
 

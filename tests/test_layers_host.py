@@ -186,6 +186,16 @@ def test_forward_without_rows_needs_nothing():
     assert lib.hip_linear_16(C.byref(linear(M=0, N=0)), None) == -1
 
 
+def test_more_workgroups_than_a_launch_holds_are_refused_before_anything_is_queued():
+    lib = ea.load()
+    big = dict(K=1 << 21, N=1 << 22, act=0, pre=None)
+    assert lib.hip_linear_16_workspace(C.byref(linear(M=(1 << 31) - 1, **big))) == -1
+    assert lib.hip_linear_16(C.byref(linear(M=(1 << 31) - 1, **big)), None) == -1
+    assert lib.hip_linear_backward_16_workspace(C.byref(linear_back(M=(1 << 31) - 1, **big))) == -1
+    assert lib.hip_experts_16_workspace(C.byref(experts(rows=(1 << 31) - 1, **big))) == -1
+    assert lib.hip_experts_backward_16_workspace(C.byref(experts_back(experts=4096, rows=100, **big))) == -1
+
+
 def test_optional_arguments():
     lib = ea.load()
     assert lib.hip_linear_16_workspace(C.byref(linear(bias=None, residual=None, pre=None))) >= 0
