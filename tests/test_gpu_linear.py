@@ -625,3 +625,55 @@ def test_torch_tensors_streams_and_graphs(gpu):
     """torch's tensors on its streams and in its graphs, in a process that torch's own runtime serves."""
     r = subprocess.run([sys.executable, "-c", TORCH % ROOT], capture_output=True, text=True, timeout=200, env=dict(os.environ))
     assert r.returncode == 0 and "OK" in r.stdout, r.stdout + r.stderr
+
+
+COLD = r"""
+import ctypes, sys
+import torch
+sys.path.insert(0, %r)
+import eshkol_amd as ea
+lib = ea.load()
+torch.manual_seed(0)
+M, K, N = 300, 256, 512
+new = lambda *s: torch.randn(*s, device="cuda").bfloat16()
+x, w, dy, y, pre, gx, gw, h, dh = new(M, K), new(K, N) * K ** -0.5, new(M, N), new(M, N), new(M, N), new(M, K), new(K, N), new(M, K), new(M, K)
+gb, mean, rstd, gg, gbeta = (torch.empty(n, device="cuda") for n in (N, M, M, K, K))
+n = ea.HipLayerNormArgs(x=x.data_ptr(), y=h.data_ptr(), mean=mean.data_ptr(), rstd=rstd.data_ptr(), rows=M, cols=K, epsilon=1e-5, dtype=3, param_dtype=3)
+f = ea.HipLinearArgs(x=h.data_ptr(), w=w.data_ptr(), y=y.data_ptr(), pre=pre.data_ptr(), M=M, K=K, N=N, dtype=3, param_dtype=3, act=3)
+b = ea.HipLinearBackwardArgs(grad_y=dy.data_ptr(), pre=pre.data_ptr(), x=h.data_ptr(), w=w.data_ptr(), grad_x=gx.data_ptr(), grad_w=gw.data_ptr(), grad_bias=gb.data_ptr(),
+                             M=M, K=K, N=N, dtype=3, grad_w_dtype=3, act=3)
+m = ea.HipLayerNormBackwardArgs(grad_y=gx.data_ptr(), x=x.data_ptr(), mean=mean.data_ptr(), rstd=rstd.data_ptr(), grad_residual=gx.data_ptr(), grad_x=dh.data_ptr(),
+                                grad_gamma=gg.data_ptr(), grad_beta=gbeta.data_ptr(), rows=M, cols=K, dtype=3, param_dtype=3)
+calls = [(lib.hip_layernorm, n), (lib.hip_linear_16, f), (lib.hip_linear_backward_16, b), (lib.hip_layernorm_backward, m)]
+room = []
+for entry, size, a in ((lib.hip_linear_16, lib.hip_linear_16_workspace, f), (lib.hip_linear_backward_16, lib.hip_linear_backward_16_workspace, b),
+                       (lib.hip_layernorm_backward, lib.hip_layernorm_backward_workspace, m)):
+    need = size(ctypes.byref(a))
+    room.append(torch.empty(max(need, 1), dtype=torch.uint8, device="cuda"))
+    a.workspace, a.workspace_bytes = room[-1].data_ptr(), need
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    for entry, a in calls:
+        assert entry(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == 0
+outs = [h, mean, rstd, y, pre, gx, gw, gb, dh, gg, gbeta]
+for turn in range(3):
+    x.copy_(new(M, K))
+    for o in outs:
+        o.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    got = [o.clone() for o in outs]
+    for entry, a in calls:
+        assert entry(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, o) for g, o in zip(got, outs)) and all(g.abs().max() > 0 for g in got)
+print("OK", flush=True)
+"""
+
+
+def test_the_first_calls_of_a_process_are_captured(gpu):
+    """Nothing has to run before a capture: a block's forward and backward pass go into a graph as a process's first calls,
+    and replay to the bits of eager calls."""
+    r = subprocess.run([sys.executable, "-c", COLD % ROOT], capture_output=True, text=True, timeout=200, env=dict(os.environ))
+    assert r.returncode == 0 and "OK" in r.stdout, r.stdout + r.stderr
