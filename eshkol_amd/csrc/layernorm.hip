@@ -80,10 +80,10 @@ __device__ __forceinline__ words_t load_vec(const E* row, uint32_t c, uint32_t n
 /* Makes the compiler take a vector's values as new ones: it would otherwise keep the widened copies of one sweep for the
  * next, in twice the registers. It also keeps the loads behind it (the parameters of this vector) from being moved up in
  * front of the sweep, all of a row's at once. */
+__device__ __forceinline__ void renew(words_t& w) { asm volatile("" : "+v"(w) :: "memory"); }
 /* A thread's place in its row, as a value of this turn of the loop: the addresses of every vector and parameter would
  * otherwise be computed once and kept, in more registers than the row itself. */
 __device__ __forceinline__ int position(int t) { asm volatile("" : "+v"(t)); return t; }
-__device__ __forceinline__ void renew(words_t& w) { asm volatile("" : "+v"(w) :: "memory"); }
 
 template <class E, class Acc, bool EVEN>
 __device__ __forceinline__ void store_vec(E* row, uint32_t c, uint32_t n, const Acc (&in)[Vec16<E>::N]) {
@@ -411,25 +411,25 @@ void norm_back_long_kernel(NormBackArgs a, const typename Elem<DT>::Acc* sums) {
 }
 
 /* grad_gamma[c] and grad_beta[c]: the sums of the n partial rows. A workgroup
- * takes 32 columns of one of the two; 8 threads share a column, each the partial
- * rows s, s + 8, ..., and their sums are added in ascending order. */
+ * takes 32 columns of one of the two; 32 threads share a column, each the partial
+ * rows s, s + 32, ..., and their sums are added in ascending order. */
 template <class Acc>
-__global__ __launch_bounds__(256)
+__global__ __launch_bounds__(1024)
 void norm_join_kernel(const Acc* __restrict__ part, uint32_t n, uint32_t cols, Acc* gg, Acc* gb) {
-    __shared__ Acc tile[8][33];
+    __shared__ Acc tile[32][33];
     Acc* out = blockIdx.y ? gb : gg;
     if (!out) return;
     const uint32_t c = blockIdx.x * 32 + (threadIdx.x & 31);
     const uint32_t s = threadIdx.x >> 5;
     Acc sum = 0;
     if (c < cols)
-#pragma unroll 8
-        for (uint32_t p = s; p < n; p += 8) sum += part[((uint64_t)p * 2 + blockIdx.y) * cols + c];
+#pragma unroll 16
+        for (uint32_t p = s; p < n; p += 32) sum += part[((uint64_t)p * 2 + blockIdx.y) * cols + c];
     tile[s][threadIdx.x & 31] = sum;
     __syncthreads();
     if (s == 0 && c < cols) {
 #pragma unroll
-        for (int k = 1; k < 8; k++) sum += tile[k][threadIdx.x];
+        for (int k = 1; k < 32; k++) sum += tile[k][threadIdx.x];
         out[c] = sum;
     }
 }
@@ -590,7 +590,7 @@ void dispatch_back(const NormBackArgs& a, const NormBackPlan& p, void* sums, voi
         else launch_back<DT, 1024, 2>(a, p.grid, st);
     }
     if (gg || gb)
-        hipLaunchKernelGGL((norm_join_kernel<Acc>), dim3((unsigned)((a.cols + 31) / 32), 2), dim3(256), 0, st,
+        hipLaunchKernelGGL((norm_join_kernel<Acc>), dim3((unsigned)((a.cols + 31) / 32), 2), dim3(1024), 0, st,
                            (const Acc*)a.part, a.rows ? (uint32_t)p.grid : 0u, a.cols, (Acc*)gg, (Acc*)gb);
 }
 
