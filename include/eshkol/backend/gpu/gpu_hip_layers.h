@@ -18,9 +18,11 @@
  * length; rows and pointers need the alignment of an element and no more
  * (16-byte aligned rows are faster). A pitch may be given as 0: the row's length.
  *
- * Memory. The calls allocate nothing, take no lock, keep nothing between calls
- * and synchronise nothing: they touch only the memory they are given, so they may
- * be called from any thread, on any stream, and be captured into a graph. Those
+ * Memory. The calls allocate nothing, synchronise nothing and keep nothing of a
+ * call: they touch only the memory they are given, so they may be called from any
+ * thread, on any stream, and be captured into a graph. (What the process does keep
+ * is which kernels have been given their LDS on which device, under a lock held for
+ * a look at that list; a kernel's first call registers it.) Those
  * that need scratch take it from the caller: fill in everything else, ask the
  * *_workspace function (host arithmetic only; -1 where the call itself would
  * refuse the arguments), and pass at least so many bytes, 16-byte aligned. Its
