@@ -150,27 +150,10 @@ __device__ __forceinline__ float sigmoid_of(float z) { return __builtin_amdgcn_r
  * the limit and not infinity times 0; NaN stays NaN */
 __device__ __forceinline__ float within(float z, float most) { return fabsf(z) > most ? __builtin_copysignf(most, z) : z; }
 
-/* z Phi(z) = max(z, 0) - |z| Phi(-|z|), Phi(-a) = exp(-a^2 / 2) (c1 t + ... + c6 t^6), t = 1 / (1 + p a): p and the
- * coefficients were fitted for the least relative error, 3.7e-6 over 0 <= a <= 13.5 (where Phi leaves the range of
- * fp32). That is 1/130 of half a step of f16, and an epilogue's vector work is not hidden behind the matrix cores of the
- * same wave. */
-__device__ __forceinline__ float gelu_of(float z) {
-    const float a = fabsf(z) > 14.0f ? 14.0f : fabsf(z);
-    const float t = __builtin_amdgcn_rcpf(fmaf(a, 0.3076693545535144f, 1.0f));
-    float p = -0.0758072764114048f;
-    p = fmaf(p, t, 0.19153177722556594f);
-    p = fmaf(p, t, 0.0054149948373767845f);
-    p = fmaf(p, t, 0.1372896528609662f);
-    p = fmaf(p, t, 0.11856265887668457f);
-    p = fmaf(p, t, 0.1230063487838367f);
-    return fmaf(-a, p * t * __builtin_amdgcn_exp2f(a * a * -0.72134752044448170f), fmaxf(z, 0.0f));
-}
-
-/* Phi(z) + z phi(z), the derivative of z Phi(z): with d = phi(a) (R(a) - a), R = Phi(-a) / phi(a), a = |z|, it is d below
- * zero and 1 - d above, one exponential for both terms. sqrt(2 pi)^-1 R is a polynomial of t = 1 / (1 + p a), fitted like the
- * one above but with eight coefficients, least relative error 8.4e-8: the bias gradient sums these unrounded. */
-__device__ __forceinline__ float gelu_slope_of(float z) {
-    const float a = fabsf(z) > 14.0f ? 14.0f : fabsf(z);
+/* Phi(-a) / phi(a) / sqrt(2 pi) for 0 <= a <= 14 (Phi the normal distribution's integral, phi its density; Phi leaves the range of
+ * fp32 at 13.5): t (c1 + c2 t + ... + c8 t^7), t = 1 / (1 + p a). p and the coefficients were fitted for the least relative error,
+ * 8.4e-8 over 0 .. 13.5; evaluated in fp32 it is within 1.5e-7 .. 7e-7. */
+__device__ __forceinline__ float normal_ratio(float a) {
     const float t = __builtin_amdgcn_rcpf(fmaf(a, 0.30401892054236973f, 1.0f));
     float p = 0.036861336417387855f;
     p = fmaf(p, t, -0.1552789393030083f);
@@ -179,8 +162,24 @@ __device__ __forceinline__ float gelu_slope_of(float z) {
     p = fmaf(p, t, 0.12352392127006696f);
     p = fmaf(p, t, 0.10243598088911153f);
     p = fmaf(p, t, 0.12217721613835655f);
-    p = fmaf(p, t, 0.12124228790163077f);
-    const float d = __builtin_amdgcn_exp2f(a * a * -0.72134752044448170f) * fmaf(p, t, a * -0.39894228040143268f);
+    return t * fmaf(p, t, 0.12124228790163077f);
+}
+/* exp(-a^2 / 2): the exponent's two roundings make a relative error of a^2 2^-24, 7e-6 where Phi leaves the range of fp32 */
+__device__ __forceinline__ float normal_exp(float a) { return __builtin_amdgcn_exp2f(a * a * -0.72134752044448170f); }
+
+/* z Phi(z) = max(z, 0) - |z| Phi(-|z|), relative error 5e-7 for |z| below 2, 7e-7 below 4. Six coefficients (3.7e-6, 9e-6 at |z| = 11)
+ * put one f16 value in 430 on the wrong side of a rounding and gained little: 8192^3 914-917 us and with these 919, the
+ * experts' 16384 rows x 1024 x 4096 244-246 and 246. */
+__device__ __forceinline__ float gelu_of(float z) {
+    const float a = fabsf(z) > 14.0f ? 14.0f : fabsf(z);
+    return fmaf(-a, normal_ratio(a) * normal_exp(a), fmaxf(z, 0.0f));
+}
+
+/* Phi(z) + z phi(z), the derivative of z Phi(z): with d = phi(a) (R(a) - a), R = Phi(-a) / phi(a), a = |z|, it is d below
+ * zero and 1 - d above, one exponential for both terms */
+__device__ __forceinline__ float gelu_slope_of(float z) {
+    const float a = fabsf(z) > 14.0f ? 14.0f : fabsf(z);
+    const float d = normal_exp(a) * fmaf(a, -0.39894228040143268f, normal_ratio(a));
     return z < 0.0f ? d : 1.0f - d;
 }
 

@@ -251,6 +251,27 @@ def test_activations_far_out(gpu, code):
     t.check_backward(None, None, gb)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=lambda t: NAMES[t])
+@pytest.mark.parametrize("M", [1, 100])
+def test_gelu_rounds_to_the_neighbour_the_formula_does(gpu, M, dtype):
+    """z Phi(z) of 2^16 sums known exactly (x is 0, so z is the fp32 bias): y is what some value within the evaluation's error of
+    the formula rounds to. That error, relative, in u: the rounding of 1 + p a and its reciprocal 3, passed on at most twofold; the
+    polynomial's steps 8; the fit 1.5; three products and the hardware's 2^x 6; the last addition 1; the exponent's two roundings
+    1.5 z^2. Together at most 24 + 2 z^2."""
+    N = 1 << 16
+    t = Layer(M, 8, N, dtype, 0, 3, F32, bias=False)
+    t.x = Mat((M, 8), dtype, values=np.zeros((M, 8)))
+    t.bias = vec(np.random.default_rng(M).uniform(-4, 4, N)[None], F32)
+    z = t.bias.values[0]
+    y, _ = t.forward(pre=False)
+    f = act(z, 3)
+    off = (24 + 2 * z * z) * U * np.abs(f)
+    least, most = decode(encode(f - off, dtype), dtype), decode(encode(f + off, dtype), dtype)
+    got = y.get()
+    bad = (got < least) | (got > most)
+    assert not bad.any(), "%d of %d values rounded from too far" % (bad.sum(), bad.size)
+
+
 def test_activations_at_the_ends_of_the_range(gpu):
     """Sums of +-infinity, of the type's largest value and NaN: the limits, and NaN."""
     big = 3.3895313892515355e38
