@@ -144,6 +144,12 @@ __device__ __forceinline__ float tanh_of(float z) {
     const float big = fmaf(-2.0f, __builtin_amdgcn_rcpf(exp_of(2.0f * a) + 1.0f), 1.0f);
     return a < 0.25f ? small : __builtin_copysignf(big, z);
 }
+/* 1 - tanh^2 z = 4 e / (1 + e)^2, e = exp(-2 |z|): no difference, so a saturated unit's derivative keeps its digits (as 1 - t^2
+ * it is 4e-4 off at |z| = 5, 6e-2 at 8 and 0 from 9 on, where it is 6e-8). Relative error (4 |z| + 11) 2^-24. */
+__device__ __forceinline__ float tanh_slope_of(float z) {
+    const float e = exp_of(-2.0f * fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + e);
+    return 4.0f * e * r * r;
+}
 __device__ __forceinline__ float sigmoid_of(float z) { return __builtin_amdgcn_rcpf(1.0f + exp_of(-z)); }
 
 /* z no further out than +-most, where the functions below have long reached their limits, so that an infinity gives
@@ -198,7 +204,7 @@ __device__ __forceinline__ void act8(float (&v)[8], int act) {
 __device__ __forceinline__ void slope8(float (&d)[8], const float (&v)[8], int act) {
 #define SLOPE(expr) do { _Pragma("unroll") for (int i = 0; i < 8; i++) { const float z = v[i]; d[i] *= (expr); } } while (0)
     switch (act) {
-    case HIP_ACT_TANH: SLOPE(({ const float t = tanh_of(z); fmaf(-t, t, 1.0f); })); break;
+    case HIP_ACT_TANH: SLOPE(tanh_slope_of(z)); break;
     case HIP_ACT_RELU: SLOPE(z > 0.0f ? 1.0f : (z != z ? z : 0.0f)); break;
     case HIP_ACT_GELU: SLOPE(gelu_slope_of(z)); break;
     case HIP_ACT_SILU: SLOPE(({ const float c = within(z, 100.0f), s = sigmoid_of(c); s * fmaf(c, 1.0f - s, 1.0f); })); break;

@@ -272,6 +272,24 @@ def test_gelu_rounds_to_the_neighbour_the_formula_does(gpu, M, dtype):
     assert not bad.any(), "%d of %d values rounded from too far" % (bad.sum(), bad.size)
 
 
+def test_the_slope_of_a_saturated_tanh_keeps_its_digits(gpu):
+    """grad_bias of one row is grad_y act'(pre): relative to 1 / cosh^2 z. The derivative is 4 e r^2, e = exp(-2 |z|),
+    r = 1 / (1 + e): e is off by 4 |z| u (two roundings of the exponent) and 2 u, r by 3 u, the products by 2 u and the one
+    with grad_y by u: 4 |z| + 11, allowed 4 |z| + 16."""
+    for dtype in (F16, BF16):
+        z = np.linspace(0, 40, 641)
+        z = decode(encode(np.concatenate([z, -z]), dtype), dtype)
+        for M in (1, 3):
+            t = Layer(M, 8, len(z), dtype, 0, 1, F32)
+            dy = np.zeros((M, len(z)))
+            dy[M - 1] = 1.5
+            t.dy = Mat(dy.shape, dtype, values=dy)
+            t.pre = Mat(dy.shape, dtype, values=np.broadcast_to(z, dy.shape))
+            got = t.backward(want="b")[2].get()[0]
+            want = 1.5 / np.cosh(z) ** 2
+            close(got, want, (4 * np.abs(z) + 16) * U * want, "slope of tanh, %s" % NAMES[dtype])
+
+
 def test_activations_at_the_ends_of_the_range(gpu):
     """Sums of +-infinity, of the type's largest value and NaN: the limits, and NaN."""
     big = 3.3895313892515355e38
