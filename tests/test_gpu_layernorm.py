@@ -113,6 +113,55 @@ def test_constant_rows_and_large_means(gpu):
     check_forward(x, None, beta, y, mean, rstd, F32)
 
 
+@pytest.mark.parametrize("cols", [3, 41, 49, 1000, 3000, 4099, 5001, 16390, 33000, 100003])
+@pytest.mark.parametrize("dtype", [F64, F32, F16, BF16], ids=lambda t: NAMES[t])
+def test_a_row_of_one_value_has_that_mean(gpu, dtype, cols):
+    """The first mean is off by at most k u of the value c, k the steps of its sum (at most cols / 1024 + 90). The deviations from it
+    are exact and equal, their mean is k u of them off, so the corrected mean is c but for (k u)^2 c, less than a quarter of c's last
+    place, and rounds to c: y is beta. The variance that is left is (k u c)^2 (2 k + 8) u."""
+    u, k = unit(dtype), cols / 1024 + 90
+    values = [1000.0, 4096.0, 0.1, 1.0, -3.7e4, 1e-3, 65504.0 / 3]
+    x = Mat((len(values), cols), dtype, values=np.repeat(np.array(values)[:, None], cols, 1))
+    c = x.values[:, 0]
+    beta = vec(np.linspace(-2, 2, cols), dtype)
+    y, mean, rstd = forward(x, None, beta, dtype, dtype)
+    assert (k * u) ** 2 < u / 4
+    assert np.array_equal(mean.get(), c)
+    assert np.array_equal(y.get(), np.broadcast_to(beta.values, x.shape))
+    want = 1e-5 ** -0.5
+    close(rstd.get(), np.full(len(c), want), want * ((k * u * c) ** 2 * (2 * k + 8) * u / 2e-5 + 4 * u), "rstd")
+
+
+@pytest.mark.parametrize("cols", [41, 700, 1000, 3000, 4099, 9000, 16390, 40000])
+@pytest.mark.parametrize("dtype", [F64, F32, BF16], ids=lambda t: NAMES[t])
+def test_statistics_beside_a_large_mean(gpu, dtype, cols):
+    """Deviations of 1 about means of a thousand and more: the mean is rounded once, and beside that off by the sum of the deviations
+    from the first mean, k + 3 roundings of their magnitudes; those are off themselves by the rounding of a difference."""
+    rng = np.random.default_rng([cols, dtype])
+    x = Mat((6, cols), dtype, values=np.array([[1000.0], [-1234.5], [3e4], [77.7], [1.0], [0.0]]) + rng.standard_normal((6, cols)))
+    y, mean, rstd = forward(x, None, None, dtype, dtype)
+    X = x.values
+    mu = X.mean(1)
+    u, k = unit(dtype), cols / 1024 + 90
+    first = k * u * np.abs(X).mean(1)                    # how far the first mean may be off
+    d = np.abs(X - mu[:, None]).mean(1) + first
+    # u for the rounding, and 2^-53 of the 64-bit mean this is held to
+    close(mean.get(), mu, u * np.abs(mu) + (k + 4) * u * d + 4 * 2.0 ** -53 * np.abs(X).mean(1), "mean")
+    check_forward(x, None, None, y, mean, rstd, dtype)
+
+
+def test_the_mean_of_a_row_with_an_infinity(gpu):
+    """The sum's own: an infinity of its sign, NaN beside the other or a NaN; y of such a row is NaN."""
+    for cols in (50, 3000, 40000):
+        v = np.random.default_rng(cols).standard_normal((5, cols))
+        v[0, 3], v[1, cols - 1], v[2, [1, 7]], v[3, 5] = np.inf, -np.inf, [np.inf, -np.inf], np.nan
+        x = Mat((5, cols), F32, values=v)
+        y, mean, rstd = forward(x, None, None, F32, F32)
+        m = mean.get()
+        assert m[0] == np.inf and m[1] == -np.inf and np.isnan(m[2:4]).all() and np.isfinite(m[4])
+        assert np.isnan(y.get()[:4]).all() and np.isnan(rstd.get()[:4]).all() and np.isfinite(y.get()[4]).all()
+
+
 def test_infinities_and_nan_stay_in_their_row(gpu):
     for cols in (50, 3000, 40000):
         rng = np.random.default_rng(cols)
