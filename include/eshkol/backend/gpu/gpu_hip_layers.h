@@ -30,9 +30,13 @@
  * same time, and two captured graphs that can, need a workspace each. Pointers must be
  * usable on the stream's device, which need not be the current one.
  *
- * Results do not depend on timing: every sum is taken in an order that the sizes
- * and the device's CU count fix. Sums, means and deviations are held in fp32 (f64
- * tensors: f64), and an output is rounded once.
+ * Results do not depend on timing: every sum is taken in an order that the call
+ * fixes, by its sizes and types, the alignment of its pointers and pitches, which
+ * outputs it asks for, and the device's CU count. The same call gives the same bits;
+ * one that asks for other outputs too, or has the same values at another alignment,
+ * may add in another order and round differently. Sums, means and deviations are
+ * held in fp32 (f64 tensors: f64), and an output is rounded once; fp32 results below
+ * 2^-119 may come out as 0 (the hardware's exponential has no subnormal results).
  */
 #ifndef ESHKOL_GPU_HIP_LAYERS_H
 #define ESHKOL_GPU_HIP_LAYERS_H
