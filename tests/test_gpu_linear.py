@@ -498,6 +498,43 @@ def test_an_expert_is_a_linear_layer(gpu):
     close(y.get(), z.get(), 2 * HALF[BF16] * np.abs(z.get()) + 1e-3, "y")          # 2 (256 + 8) u times magnitudes of about 20, twice
 
 
+# ---- whole numbers ------------------------------------------------------------------------------------------------
+
+# (rows, K, N, offsets): every kernel and cut: K whole in a workgroup, the streaming kernel with parts, tiles of 32 and 64 rows, the
+# larger tiles, with K cut and whole, blocks that end inside; experts of few rows, of many, with none
+WHOLE = [(1, 4096, 3000, None), (3, 4099, 2800, None), (2, 4096, 520, None), (13, 5000, 264, None), (30, 4104, 264, None), (60, 4096, 136, None), (37, 4101, 130, None),
+         (130, 4097, 200, None), (300, 2056, 520, None), (2048, 264, 1536, None), (2300, 200, 2304, None), (4200, 72, 3600, None), (150, 1024, 4096, None),
+         (40, 4104, 136, [0, 3, 3, 40]), (45, 4101, 130, [2, 17, 17, 18, 44]), (200, 2056, 264, list(range(0, 200, 50)) + [200]), (1500, 1032, 264, [0, 1, 700, 700, 1499]),
+         (6000, 136, 1400, [0] + list(range(100, 6000, 200)) + [6000])]
+
+
+@pytest.mark.parametrize("trans", [0, 1])
+@pytest.mark.parametrize("case", WHOLE, ids=lambda c: "%d x %d x %d%s" % (c[:3] + (", %d experts" % (len(c[3]) - 1) if c[3] else "",)))
+def test_whole_numbers_are_exact(gpu, case, trans):
+    """Operands of -1, 0 and 1 and a whole bias: every product and every partial sum is a whole number below 2^24, exact in fp32 in
+    any order, so each output is the rounding of the exact one, and one product lost or taken twice shows. (A sum of K or rows
+    products stays below 6000.)"""
+    M, K, N, offsets = case
+    dtype = BF16 if (M + trans) % 2 else F16
+    print("case: whole numbers", case, NAMES[dtype], trans, flush=True)
+    t = Layer(M, K, N, dtype, trans, 0, F32, offsets=offsets, seed=4)
+    rng = np.random.default_rng([M, K, N, trans])
+    ones = lambda shape: Mat(shape, dtype, values=rng.integers(-1, 2, shape))  # noqa: E731
+    t.x, t.w, t.dy = ones((M, K)), ones(t.w.shape), ones((M, N))
+    t.bias = vec(rng.integers(-3, 4, (t.E, N)), F32)
+    X, W, DY, B = (v.astype(np.float32) for v in (t.x.values, t.W(), t.dy.values, t.bias.values.reshape(t.E, N)))
+    y = t.forward(pre=False)[0].get()
+    gx, gw, gb = t.backward(F32)
+    gx, gw, gb = gx.get(), gw.get().reshape(t.w.shape), gb.get()
+    rounded = lambda v: decode(encode(v, dtype), dtype)  # noqa: E731
+    for e, (a, b) in enumerate(t.groups()):
+        # these sums are exact in fp32 as well
+        assert np.array_equal(y[a:b], rounded(X[a:b] @ W[e] + B[e])), "y, expert %d" % e
+        assert np.array_equal(gx[a:b], rounded(DY[a:b] @ W[e].T)), "grad_x, expert %d" % e
+        assert np.array_equal(gw[e].T if trans else gw[e], X[a:b].T @ DY[a:b]), "grad_w, expert %d" % e
+        assert np.array_equal(gb[e], DY[a:b].sum(0)), "grad_bias, expert %d" % e
+
+
 # ---- gradients against differences ---------------------------------------------------------------------------------
 
 def test_gradients_against_differences(gpu):
