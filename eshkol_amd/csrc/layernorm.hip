@@ -16,10 +16,11 @@
  * a second launch, in ascending order.
  *
  * Bound by memory: every value is read once and written once. 32768 x 4096 bf16,
- * with a device copy's 5.1 TB/s as the floor: forward 121 us (4.4 TB/s, floor 105),
+ * with a device copy's 5.1 TB/s as the floor: forward 122 us (4.4 TB/s, floor 105; f32
+ * 223, floor 211; 16384 x 4096 f64 202, floor 211),
  * backward with the residual's gradient 224 us (4.8 TB/s, floor 210; 7 of them the
  * second launch). 4095 x 1023 fp32 backward 19.5 us (floor 10): two rows per wave,
- * so the launches and the first trip to memory are half of it. One row of 4096: 3.3
+ * so the launches and the first trip to memory are half of it. One row of 4096: 3.6
  * us on the device.
  */
 #include "layer_common.h"

@@ -16,8 +16,8 @@
  * writes lanes in order, so it is the global address that is permuted. Measured: one
  * LDS cycle in a hundred is a conflict, all of them the epilogue's.
  *
- * What bounds the tiles. 8192^3 with the 256 x 256 tile: 820-860 us (1.28-1.34
- * PFLOP/s), the matrix pipe busy 67 per cent of the time; without its loads the loop
+ * What bounds the tiles. 8192^3 with the 256 x 256 tile, no epilogue: 820-860 us
+ * (1.28-1.34 PFLOP/s; with bias, gelu and pre 865-920), the matrix pipe busy 67 per cent of the time; without its loads the loop
  * takes 670 us, without its multiplications 680: operand blocks arrive in the L2 from
  * behind it at the rate at which they are multiplied, and what is lost is where the
  * two wait for each other. More blocks in flight (four and five of 32 k) gained
@@ -565,8 +565,9 @@ void linear_thin_kernel(LinearArgs g) {
 /* ---- a few rows, K whole in a workgroup: no parts, no second launch ------------------------------------------------
  * Sixteen waves share K and join in LDS; a workgroup's columns are few, so that there are workgroups enough.
  *
- * k contiguous (W [N][K]), up to sixteen rows: 16 columns, a wave takes every sixteenth 64 k. One row, K = N = 4096, bf16:
- * 7.2 us, the kernel above 6.6 and its second launch 4. */
+ * k contiguous (W [N][K]), up to sixteen rows: 16 columns, a wave takes every sixteenth 64 k. K = N = 4096, bf16, the weights
+ * of 44 layers in turn, so that they come from memory: one row 9.9 us, sixteen 12.2; the kernel above with its second launch
+ * 15.4 and 16.4. */
 template <bool BF16>
 __global__ __launch_bounds__(1024)
 void linear_few_rows_kernel(LinearArgs g) {
@@ -603,8 +604,10 @@ void linear_few_rows_kernel(LinearArgs g) {
     finish_row8<BF16>(g.e, g.e.y, row, col, g.N, v, bias);
 }
 
-/* Columns contiguous (W [K][N]), up to four rows: 32 columns (one row, K = N = 4096, bf16: 7.7 us, the kernel above 5.0 and
- * its second launch 4). A lane holds 8 k of 8 columns (transposed in its registers
+/* Columns contiguous (W [K][N]), up to four rows: 32 columns. One row, K = N = 4096, bf16: 10.7 us where the last-level cache
+ * holds W (the kernel above with its second launch 12.4), but 17.9 against 14.0 with the weights of 44 layers in turn, which come
+ * from memory. It is ahead there too up to K = 2048 (11.1 both; K = 1024: 7.5 against 9.0) and where N is no multiple of 128 (4160:
+ * 14.3 against 21.9). A lane holds 8 k of 8 columns (transposed in its registers
  * as above), and of a wave's 128 k lane l holds the sixteenth l / 4. The MFMA wants one k for all of its sixteen positions,
  * so four of them, q = l / 4 % 4, carry the same columns at different k, and the other operand's sixteen positions are four
  * rows at each of those four k: the blocks where the two q agree are the sums, the others are not looked at. */
@@ -738,6 +741,10 @@ __device__ __forceinline__ void align_rows(const AlignArgs& a, uint32_t block) {
     }
 }
 
+/* dz is rounded to the 16-bit type: it is an operand of the matrix cores. That adds its half step to the ones that x, w and the
+ * outputs were rounded with: grad_x and grad_w are 2.3e-3 off the 64-bit formula in the 2-norm instead of 1.7e-3 (bf16; f16 2.9e-4
+ * and 2.1e-4). A second operand for what the rounding leaves would double both products. The bias gradient needs no operand and
+ * sums the unrounded values. */
 template <bool BF16>
 __device__ __forceinline__ void slope_rows(const SlopeArgs& a, uint32_t block, float (*sums)[32][9]) {
     typedef typename Half16<BF16>::T E;

@@ -14,7 +14,9 @@ Matrix matrix_of(const void* p, uint64_t ld, uint64_t stride, uint64_t rows, uin
     if (m.copy) m.copy_bytes = round_up_sz((size_t)(count * rows * round_up_sz(cols, 8) * 2), 256);
     return m;
 }
-/* How a product is run. Up to sixteen rows (on average, by expert) B is streamed past them, up to 64 in tiles of 32 or 64
+/* How a product is run. Up to sixteen rows (on average, by expert: the groups' sizes are on the device) B is streamed past them,
+ * sixteen at a time, so an expert with many more is late: 1024 rows of 64 experts, 1024 x 4096, take 107 us at 16 each, 371 with 512
+ * on one and 549 with all on one. Up to 64 rows in tiles of 32 or 64
  * rows: the streaming kernel's loads of more rows outgrow those of B (K = N = 4096, W [N][K], bf16, us without the second
  * launch: 32 rows 11.3 and 7.6, 64 rows 16.9 and 8.4; one row 6.6 and 7.6). The tiles want aligned operands, and a copy of
  * B would cost more than they gain. */
@@ -52,7 +54,8 @@ void split_product(Product* q, uint64_t want, uint64_t least) {
     q->part_ld = (uint32_t)round_up_sz((size_t)q->s.N, 8);
     q->part_bytes = round_up_sz((size_t)(splits * q->s.M * q->part_ld * 4), 256);
 }
-/* The tile of one or two products launched together, and how their K is cut. Times are of bf16 products, us.
+/* The tile of one or two products launched together, and how their K is cut. Times are of bf16 products without an epilogue, us,
+ * those of one comparison from one run.
  * 256 x 256 where at least three quarters of the CUs get one (8192^3: 819; 128 x 256 921, 128 x 128 1170), products of one
  * matrix only: the last rows of a group leave half a tile empty on average.
  * 128 x 256 where that many of those there are (the two products of 4096 x 1024 x 4096: 74, 128 x 128 79; 16384 rows of 64

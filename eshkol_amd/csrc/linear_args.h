@@ -158,7 +158,7 @@ __device__ __forceinline__ float within(float z, float most) { return fabsf(z) >
 
 /* Phi(-a) / phi(a) / sqrt(2 pi) for 0 <= a <= 14 (Phi the normal distribution's integral, phi its density; Phi leaves the range of
  * fp32 at 13.5): t (c1 + c2 t + ... + c8 t^7), t = 1 / (1 + p a). p and the coefficients were fitted for the least relative error,
- * 8.4e-8 over 0 .. 13.5; evaluated in fp32 it is within 1.5e-7 .. 7e-7. */
+ * 8.4e-8 over 0 .. 13.5; evaluated in fp32 4e-7. */
 __device__ __forceinline__ float normal_ratio(float a) {
     const float t = __builtin_amdgcn_rcpf(fmaf(a, 0.30401892054236973f, 1.0f));
     float p = 0.036861336417387855f;
@@ -170,7 +170,7 @@ __device__ __forceinline__ float normal_ratio(float a) {
     p = fmaf(p, t, 0.12217721613835655f);
     return t * fmaf(p, t, 0.12124228790163077f);
 }
-/* exp(-a^2 / 2): the exponent's two roundings make a relative error of a^2 2^-24, 7e-6 where Phi leaves the range of fp32 */
+/* exp(-a^2 / 2): the exponent's two roundings make a relative error of up to a^2 2^-24 */
 __device__ __forceinline__ float normal_exp(float a) { return __builtin_amdgcn_exp2f(a * a * -0.72134752044448170f); }
 
 /* z Phi(z) = max(z, 0) - |z| Phi(-|z|), relative error 5e-7 for |z| below 2, 7e-7 below 4. Six coefficients (3.7e-6, 9e-6 at |z| = 11)
